@@ -1,0 +1,702 @@
+// Routing of tokens to experts: from a row of router logits to the chosen
+// experts and their weights, the step before moe_align / moe_gemm, and its
+// gradient.
+//
+//   s = softmax(x) or sigmoid(x)           (over the E experts of a row)
+//   c = s + bias                           (bias steers the choice only)
+//   keep the topk_groups groups with the largest sum of their group_top best c
+//   choose the topk largest c of them, largest first, ties to the lowest index
+//   w = scale * s[chosen]                  (renorm: divided by the sum of the chosen s)
+//
+// An expert whose logit is -inf or NaN, or whose c is, cannot be chosen; a
+// place that no expert is left for gets id -1 and weight 0.
+//
+// The choice is the one of exact arithmetic. Without a bias the experts of a
+// row rank as their logits do, which needs no arithmetic. With a bias, and
+// between groups, c is computed in 32 bits first; where two values that decide
+// the order are closer than those 32 bits tell apart (a few rows in a
+// thousand), the row is ranked again in 64 bits.
+//
+// A row belongs to LANES lanes of a warp, NV neighbouring experts to a lane, so
+// that a tie goes to the first lane and the first register. Each choice is one
+// maximum over the lanes and a rescan of the winner's NV registers. Rows of up
+// to 64 experts take 8 lanes (four rows per warp).
+#include "ctb_common.cuh"
+
+#include <algorithm>
+
+namespace ctb {
+namespace {
+
+constexpr int ROUTE_THREADS = 128;
+constexpr int ROUTE_MAX_EXPERTS = 256;
+constexpr int ROUTE_MAX_TOPK = 32;
+constexpr unsigned FULL = 0xffffffffu;
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void store_as(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// A run of up to 16 bytes of T.
+template <int BYTES> struct Raw;
+template <> struct Raw<2> { using type = uint16_t; };
+template <> struct Raw<4> { using type = uint32_t; };
+template <> struct Raw<8> { using type = uint2; };
+template <> struct Raw<16> { using type = uint4; };
+
+// NV neighbouring values of a row, as vectors of at most 16 bytes where VEC.
+template <typename T, int NV, bool VEC>
+__device__ __forceinline__ void load_run(const T* __restrict__ p, int i0, int E, float pad,
+                                         float (&v)[NV]) {
+  if (VEC) {
+    constexpr int W = NV * (int)sizeof(T) < 16 ? NV : 16 / (int)sizeof(T);
+    using R = typename Raw<W * (int)sizeof(T)>::type;
+#pragma unroll
+    for (int c = 0; c < NV; c += W) {
+      if (i0 < E) {  // E is a multiple of NV on this path
+        union {
+          R raw;
+          T e[W];
+        } u;
+        u.raw = *reinterpret_cast<const R*>(p + i0 + c);
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[c + i] = to_float(u.e[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[c + i] = pad;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = i0 + i < E ? to_float(p[i0 + i]) : pad;
+  }
+}
+template <typename T, int NV, bool VEC>
+__device__ __forceinline__ void store_run(T* __restrict__ p, int i0, int E, const float (&v)[NV]) {
+  if (VEC) {
+    constexpr int W = NV * (int)sizeof(T) < 16 ? NV : 16 / (int)sizeof(T);
+    using R = typename Raw<W * (int)sizeof(T)>::type;
+    if (i0 < E) {
+#pragma unroll
+      for (int c = 0; c < NV; c += W) {
+        union {
+          R raw;
+          T e[W];
+        } u;
+#pragma unroll
+        for (int i = 0; i < W; ++i) store_as(&u.e[i], v[c + i]);
+        *reinterpret_cast<R*>(p + i0 + c) = u.raw;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i0 + i < E) store_as(&p[i0 + i], v[i]);
+  }
+}
+
+// ---- reductions over the LANES lanes of a row ------------------------------------
+template <int LANES>
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+  return v;
+}
+template <int LANES, typename S>
+__device__ __forceinline__ S row_sum(S v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+
+// ---- order-preserving keys: 0 is "not available" -----------------------------------
+// Adding +0 first makes -0 and +0 the same key.
+__device__ __forceinline__ uint32_t key_of(float v) {
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t key_of(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
+  return u >> 63 ? ~u : u | (1ull << 63);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+template <typename S> struct KeyOf;
+template <> struct KeyOf<float> { using type = uint32_t; };
+template <> struct KeyOf<double> { using type = uint64_t; };
+
+template <int LANES>
+__device__ __forceinline__ uint32_t row_max_key(uint32_t v) {
+  if (LANES == 32) return __reduce_max_sync(FULL, v);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL, v, o));
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ uint64_t row_max_key(uint64_t v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    const uint64_t w = __shfl_xor_sync(FULL, v, o);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+struct RouteArgs {
+  const float* bias;
+  float* weights;
+  int32_t* ids;
+  int T, E, topk;
+  int64_t ldx;
+  int sigmoid, groups, topk_groups, group_top, renorm;
+  float scale;
+};
+
+// Whether two choice values hi >= lo are too close for 32 bits to order them.
+// __expf is documented to 2 + 1.16 |d| ulp, so exp(d) carries at most 2.4e-7 +
+// 2e-7 |d| relative error with the rounding of d; the row's sum (its terms'
+// errors weighted, 8 levels of additions) at most 2e-6, the division 2.4e-7.
+// With a bias, the scores of a pair (or of two groups) of one row err by at
+// most 4e-6 together (softmax: they add up to at most 1; sigmoid: under 6e-7
+// each), and each addition by 2^-24 of the magnitude `mag`. Without one the
+// error is relative, |ln hi| standing for |d|; sums so small that 32 bits lose
+// them are never certain.
+__device__ __forceinline__ bool too_close_biased(float hi, float lo, float mag) {
+  return !(hi - lo > 4e-6f + 5e-7f * mag);
+}
+__device__ __forceinline__ bool too_close_unbiased(float hi, float lo) {
+  return !(hi > 1e-30f && hi - lo > 2.f * hi * (4e-6f + 2.5e-7f * fabsf(__logf(hi))));
+}
+
+// Keys of the experts outside the best topk_groups groups become 0; returns
+// whether the choice between groups was too close for 32 bits. LANES == 32.
+template <typename S, int NV>
+__device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV],
+                                            typename KeyOf<S>::type (&key)[NV], S* row) {
+  const int lane = threadIdx.x & 31, size = a.E / a.groups;
+  const S none = -INFINITY;
+  S best = none, second = none;
+  const int span = size / NV;  // lanes per group
+  if (size % NV == 0 && (span & (span - 1)) == 0) {
+    // Whole lanes per group: the two best of a lane's registers, then of neighbours.
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const S x = key[v] ? c[v] : none;
+      second = max(second, min(best, x));
+      best = max(best, x);
+    }
+    for (int o = 1; o < span; o <<= 1) {
+      const S b = __shfl_xor_sync(FULL, best, o), s = __shfl_xor_sync(FULL, second, o);
+      second = max(max(second, s), min(best, b));
+      best = max(best, b);
+    }
+    const int from = min(lane * span, 31);
+    best = __shfl_sync(FULL, best, from);
+    second = __shfl_sync(FULL, second, from);
+  } else {
+    // Through shared memory; one word in 32 is skipped so that lanes that
+    // start a multiple of 32 apart use different banks.
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = lane * NV + v;
+      if (i < a.E) row[i + (i >> 5)] = key[v] ? c[v] : none;
+    }
+    __syncwarp();
+    if (lane < a.groups)
+      for (int i = lane * size; i < (lane + 1) * size; ++i) {
+        const S x = row[i + (i >> 5)];
+        second = max(second, min(best, x));
+        best = max(best, x);
+      }
+    __syncwarp();
+  }
+  S score = best;
+  if (a.group_top > 1 && second > none) score = best + second;
+  if (lane >= a.groups) score = none;
+  int rank = 0;
+  for (int g = 0; g < a.groups; ++g) {
+    const S o = __shfl_sync(FULL, score, g);
+    rank += o > score || (o == score && g < lane);
+  }
+  const bool in = lane < a.groups && rank < a.topk_groups;
+  const unsigned kept = __ballot_sync(FULL, in);
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int i = lane * NV + v;
+    if (i < a.E && !(kept >> (i / size) & 1u)) key[v] = 0;
+  }
+  bool close = false;
+  if (sizeof(S) == 4) {
+    const uint32_t k = key_of((float)score);
+    const float lo = value_of(__reduce_min_sync(FULL, in ? k : 0xffffffffu));
+    const float hi = value_of(__reduce_max_sync(FULL, lane < a.groups && !in ? k : 0u));
+    const float size_of = lane < a.groups && best > none
+                              ? fabsf((float)best) + (second > none ? fabsf((float)second) : 0.f)
+                              : 0.f;
+    const float mag = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(size_of)));
+    // A group without an expert (-inf) is not in doubt.
+    close = hi > -INFINITY &&
+            (a.bias ? too_close_biased(lo, hi, mag) : too_close_unbiased(lo, hi));
+  }
+  return close;
+}
+
+// Writes the chosen experts to sel[0..topk); with `check`, returns whether two
+// neighbours in the order (the first one left out included) were too close.
+template <typename K, int LANES, int NV>
+__device__ __forceinline__ bool choose(const RouteArgs& a, K (&key)[NV], int* sel, bool check) {
+  const int lane = threadIdx.x & 31, sub = lane % LANES, base = lane - sub;
+  bool close = false;
+  float before = INFINITY;
+  const int rounds = a.topk + (check ? 1 : 0);
+  K kb = 0;
+  int vb = 0;
+  auto rescan = [&] {
+    kb = key[0];
+    vb = 0;
+#pragma unroll
+    for (int v = 1; v < NV; ++v)
+      if (key[v] > kb) {
+        kb = key[v];
+        vb = v;
+      }
+  };
+  rescan();
+  for (int j = 0; j < rounds; ++j) {
+    const K m = row_max_key<LANES>(kb);
+    const unsigned who = __ballot_sync(FULL, kb == m) >> base;
+    const int win = __ffs(LANES == 32 ? who : who & ((1u << (LANES & 31)) - 1u)) - 1;
+    if (check) {
+      const float v = m ? value_of((uint32_t)m) : -INFINITY;
+      if (m && j > 0) close |= too_close_biased(before, v, fabsf(before) + fabsf(v));
+      before = v;
+    }
+    if (sub == win) {
+      if (j < a.topk) sel[j] = m ? sub * NV + vb : -1;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if (v == vb) key[v] = 0;
+      rescan();
+    }
+  }
+  __syncwarp();
+  return close;
+}
+
+// The same row ranked in 64 bits.
+template <typename T, int LANES, int NV, bool GROUPED>
+__device__ __noinline__ void choose_exact(const RouteArgs& a, const T* __restrict__ x, int i0,
+                                          bool in_range, int* sel, double* row) {
+  double c[NV];
+  uint64_t key[NV];
+  double top = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    c[v] = in_range && i0 + v < a.E ? (double)to_float(x[i0 + v]) : -INFINITY;
+    if (isnan(c[v])) c[v] = -INFINITY;
+    top = max(top, c[v]);
+  }
+  double total = 1.0;
+  if (!a.sigmoid) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(FULL, top, o));
+    if (top == -INFINITY) top = 0.0;
+    total = 0.0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) total += exp(c[v] - top);
+    total = row_sum<LANES>(total);
+  }
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const double xv = c[v];
+    const double s = a.sigmoid ? 1.0 / (1.0 + exp(-xv)) : exp(xv - top) / total;
+    c[v] = a.bias && i0 + v < a.E ? s + (double)a.bias[i0 + v] : s;
+    const bool live = xv > -INFINITY && c[v] > -INFINITY;
+    key[v] = live ? key_of(a.bias ? c[v] : xv) : 0;
+  }
+  if (GROUPED) keep_groups<double, NV>(a, c, key, row);
+  choose<uint64_t, LANES, NV>(a, key, sel, false);
+}
+
+template <typename T, int LANES, int NV, bool VEC, bool GROUPED>
+__global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __restrict__ x,
+                                                                  const RouteArgs a) {
+  constexpr int ROWS = ROUTE_THREADS / LANES;
+  constexpr int SLOTS = ROUTE_MAX_TOPK / LANES;  // places of a row per lane
+  __shared__ int sel_all[ROWS][ROUTE_MAX_TOPK];
+  __shared__ double scratch[GROUPED ? ROUTE_THREADS / 32 : 1]
+                           [GROUPED ? ROUTE_MAX_EXPERTS + ROUTE_MAX_EXPERTS / 32 : 1];
+  const int lane = threadIdx.x & 31, sub = lane % LANES, r = threadIdx.x / LANES;
+  const int64_t t = (int64_t)blockIdx.x * ROWS + r;
+  const bool in_range = t < a.T;
+  const T* xr = x + (in_range ? t : 0) * a.ldx;
+  int* sel = sel_all[r];
+  const int i0 = sub * NV;
+
+  float xv[NV];
+  load_run<T, NV, VEC>(xr, i0, in_range ? a.E : 0, -INFINITY, xv);
+  float top = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if (isnan(xv[v])) xv[v] = -INFINITY;
+    top = fmaxf(top, xv[v]);
+  }
+  // Softmax over the row, where the choice or the weights need it.
+  float total = 1.f;
+  const bool scores = a.bias != nullptr || GROUPED;
+  if (!a.sigmoid && (scores || !a.renorm)) {
+    top = row_max<LANES>(top);
+    if (top == -INFINITY) top = 0.f;
+    total = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) total += __expf(xv[v] - top);
+    total = row_sum<LANES>(total);
+  }
+  float c[NV];
+  uint32_t key[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    c[v] = xv[v];
+    if (scores) {
+      const float s = a.sigmoid ? __fdividef(1.f, 1.f + __expf(-xv[v]))
+                                : __fdividef(__expf(xv[v] - top), total);
+      c[v] = a.bias && i0 + v < a.E ? s + a.bias[i0 + v] : s;
+    }
+    const bool live = xv[v] > -INFINITY && c[v] > -INFINITY;
+    key[v] = live ? key_of(a.bias ? c[v] : xv[v]) : 0u;
+  }
+  bool close = false;
+  double* row = scratch[GROUPED ? threadIdx.x / 32 : 0];
+  if (GROUPED) close = keep_groups<float, NV>(a, c, key, reinterpret_cast<float*>(row));
+  close |= choose<uint32_t, LANES, NV>(a, key, sel, a.bias != nullptr);
+  if (__any_sync(FULL, close && in_range))
+    choose_exact<T, LANES, NV, GROUPED>(a, xr, i0, in_range, sel, row);
+
+  // Weights: place j belongs to lane j % LANES of its row.
+  float xs[SLOTS], w[SLOTS];
+  int id[SLOTS];
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const int j = sub + i * LANES;
+    id[i] = in_range && j < a.topk ? sel[j] : -1;
+    xs[i] = id[i] >= 0 ? to_float(xr[id[i]]) : -INFINITY;
+    m = fmaxf(m, xs[i]);
+  }
+  if (a.renorm) {
+    // The common factor exp(-m) (sigmoid: exp(-min(m, 0))) leaves the shares as
+    // they are and keeps them exact where all scores of a row underflow.
+    m = row_max<LANES>(m);
+    const float shift = a.sigmoid ? fminf(m, 0.f) : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      w[i] = 0.f;
+      if (id[i] >= 0) {
+        w[i] = a.sigmoid && xs[i] > 0.f ? 1.f : expf(xs[i] - shift);
+        if (a.sigmoid) w[i] /= 1.f + expf(-fabsf(xs[i]));
+      }
+      sum += w[i];
+    }
+    sum = row_sum<LANES>(sum);
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) w[i] = id[i] >= 0 ? w[i] / sum : 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i)
+      w[i] = id[i] < 0 ? 0.f
+                       : a.sigmoid ? 1.f / (1.f + expf(-xs[i])) : expf(xs[i] - top) / total;
+  }
+  if (in_range) {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int j = sub + i * LANES;
+      if (j < a.topk) {
+        a.weights[t * a.topk + j] = w[i] * a.scale;
+        a.ids[t * a.topk + j] = id[i];
+      }
+    }
+  }
+}
+
+// -----------------------------------------------------------------------------
+// Gradient of the weights with respect to the logits (the choice itself and the
+// bias have none). With g = scale * dw, s the scores and p = s / sum(chosen s):
+//   softmax         dx = s * (g - sum(g s))              over the whole row
+//   softmax, renorm dx = p * (g - sum(g p))              chosen experts only
+//   sigmoid         dx = g s (1 - s)                     chosen experts only
+//   sigmoid, renorm dx = p (1 - s) * (g - sum(g p))      chosen experts only
+// One pass: the row (plain softmax) or the chosen logits are read, the whole
+// row of dx is written once.
+// -----------------------------------------------------------------------------
+struct RouteBwdArgs {
+  const float* dweights;
+  const int32_t* ids;
+  int T, E, topk;
+  int64_t ldx, lddx;
+  int sigmoid, renorm;
+  float scale;
+};
+
+template <typename T, int LANES, int NV, bool VEC>
+__global__ void __launch_bounds__(ROUTE_THREADS)
+    moe_route_bwd_kernel(const T* __restrict__ x, T* __restrict__ dx, const RouteBwdArgs a) {
+  constexpr int ROWS = ROUTE_THREADS / LANES;
+  constexpr int SLOTS = ROUTE_MAX_TOPK / LANES;
+  __shared__ int2 slot_all[ROWS][ROUTE_MAX_TOPK];  // (expert, gradient bits) of each place
+  const int lane = threadIdx.x & 31, sub = lane % LANES, r = threadIdx.x / LANES;
+  const int64_t t = (int64_t)blockIdx.x * ROWS + r;
+  const bool in_range = t < a.T;
+  const T* xr = x + (in_range ? t : 0) * a.ldx;
+  int2* slot = slot_all[r];
+  const int i0 = sub * NV;
+
+  const bool whole = !a.sigmoid && !a.renorm;
+  float xv[NV], top = -INFINITY, total = 1.f;
+  if (whole) {
+    load_run<T, NV, VEC>(xr, i0, in_range ? a.E : 0, -INFINITY, xv);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (isnan(xv[v])) xv[v] = -INFINITY;
+      top = fmaxf(top, xv[v]);
+    }
+    top = row_max<LANES>(top);
+    if (top == -INFINITY) top = 0.f;
+    total = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      xv[v] = expf(xv[v] - top);
+      total += xv[v];
+    }
+    total = row_sum<LANES>(total);
+    if (!(total > 0.f)) total = 1.f;
+  }
+  float xs[SLOTS], g[SLOTS], p[SLOTS];
+  int id[SLOTS];
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const int j = sub + i * LANES;
+    id[i] = in_range && j < a.topk ? a.ids[t * a.topk + j] : -1;
+    if (id[i] >= a.E) id[i] = -1;
+    xs[i] = id[i] >= 0 ? to_float(xr[id[i]]) : -INFINITY;
+    if (isnan(xs[i])) xs[i] = -INFINITY;
+    if (xs[i] == -INFINITY) id[i] = -1;  // no share, no gradient
+    g[i] = id[i] >= 0 ? a.dweights[t * a.topk + j] * a.scale : 0.f;
+    m = fmaxf(m, xs[i]);
+  }
+  if (a.renorm) {
+    m = row_max<LANES>(m);
+    const float shift = a.sigmoid ? fminf(m, 0.f) : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      p[i] = 0.f;
+      if (id[i] >= 0) {
+        p[i] = a.sigmoid && xs[i] > 0.f ? 1.f : expf(xs[i] - shift);
+        if (a.sigmoid) p[i] /= 1.f + expf(-fabsf(xs[i]));
+      }
+      sum += p[i];
+    }
+    sum = row_sum<LANES>(sum);
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      p[i] *= inv;
+      dot += g[i] * p[i];
+    }
+    dot = row_sum<LANES>(dot);
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      g[i] = p[i] * (g[i] - dot);
+      if (a.sigmoid) g[i] /= 1.f + expf(xs[i]);
+    }
+  } else if (a.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const float e = expf(-fabsf(xs[i]));  // s (1 - s) = e / (1 + e)^2, either sign of x
+      if (id[i] >= 0) g[i] *= e / ((1.f + e) * (1.f + e));
+    }
+  } else {
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      if (id[i] >= 0) g[i] *= expf(xs[i] - top) / total;
+      dot += g[i];
+    }
+    dot = row_sum<LANES>(dot);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) xv[v] *= -dot / total;
+  }
+  if (!whole) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) xv[v] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const int j = sub + i * LANES;
+    if (j < a.topk) slot[j] = make_int2(id[i], __float_as_int(g[i]));
+  }
+  __syncwarp();
+  for (int j = 0; j < a.topk; ++j) {
+    const int2 s = slot[j];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (s.x == i0 + v) xv[v] += __int_as_float(s.y);
+  }
+  if (in_range) store_run<T, NV, VEC>(dx + t * a.lddx, i0, a.E, xv);
+}
+
+// ---- host ----------------------------------------------------------------------
+// Whether rows of T can move as NV-wide vectors of at most 16 bytes.
+template <typename T>
+bool runs_ok(const void* p, int64_t ld, int E, int NV) {
+  const int64_t bytes = std::min<int64_t>(16, NV * (int64_t)sizeof(T));
+  return E % NV == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0 &&
+         (ld * (int64_t)sizeof(T)) % bytes == 0;
+}
+
+template <typename T, int LANES, int NV, bool GROUPED>
+int route_launch(const T* x, const RouteArgs& a, cudaStream_t st) {
+  const int rows = ROUTE_THREADS / LANES;
+  const unsigned grid = (unsigned)(((int64_t)a.T + rows - 1) / rows);
+  if (runs_ok<T>(x, a.ldx, a.E, NV))
+    moe_route_kernel<T, LANES, NV, true, GROUPED><<<grid, ROUTE_THREADS, 0, st>>>(x, a);
+  else
+    moe_route_kernel<T, LANES, NV, false, GROUPED><<<grid, ROUTE_THREADS, 0, st>>>(x, a);
+  return launch_status("moe_route_kernel");
+}
+template <typename T>
+int route_dispatch(const T* x, const RouteArgs& a, cudaStream_t st) {
+  if (a.topk_groups < a.groups) {  // a group per lane: always a whole warp per row
+    if (a.E <= 32) return route_launch<T, 32, 1, true>(x, a, st);
+    if (a.E <= 64) return route_launch<T, 32, 2, true>(x, a, st);
+    if (a.E <= 128) return route_launch<T, 32, 4, true>(x, a, st);
+    return route_launch<T, 32, 8, true>(x, a, st);
+  }
+  if (a.E <= 8) return route_launch<T, 8, 1, false>(x, a, st);
+  if (a.E <= 16) return route_launch<T, 8, 2, false>(x, a, st);
+  if (a.E <= 32) return route_launch<T, 8, 4, false>(x, a, st);
+  if (a.E <= 64) return route_launch<T, 8, 8, false>(x, a, st);
+  if (a.E <= 128) return route_launch<T, 16, 8, false>(x, a, st);
+  return route_launch<T, 32, 8, false>(x, a, st);
+}
+
+template <typename T, int LANES, int NV>
+int route_bwd_launch(const T* x, T* dx, const RouteBwdArgs& a, cudaStream_t st) {
+  const int rows = ROUTE_THREADS / LANES;
+  const unsigned grid = (unsigned)(((int64_t)a.T + rows - 1) / rows);
+  if (runs_ok<T>(x, a.ldx, a.E, NV) && runs_ok<T>(dx, a.lddx, a.E, NV))
+    moe_route_bwd_kernel<T, LANES, NV, true><<<grid, ROUTE_THREADS, 0, st>>>(x, dx, a);
+  else
+    moe_route_bwd_kernel<T, LANES, NV, false><<<grid, ROUTE_THREADS, 0, st>>>(x, dx, a);
+  return launch_status("moe_route_bwd_kernel");
+}
+template <typename T>
+int route_bwd_dispatch(const T* x, T* dx, const RouteBwdArgs& a, cudaStream_t st) {
+  if (a.E <= 8) return route_bwd_launch<T, 8, 1>(x, dx, a, st);
+  if (a.E <= 16) return route_bwd_launch<T, 8, 2>(x, dx, a, st);
+  if (a.E <= 32) return route_bwd_launch<T, 8, 4>(x, dx, a, st);
+  if (a.E <= 64) return route_bwd_launch<T, 8, 8>(x, dx, a, st);
+  if (a.E <= 128) return route_bwd_launch<T, 16, 8>(x, dx, a, st);
+  return route_bwd_launch<T, 32, 8>(x, dx, a, st);
+}
+
+// What both directions check; `k` names the entry point.
+int route_check(const char* k, int dtype, int T, int E, int topk, int64_t ldx, int score) {
+  const std::string n(k);
+  if (dtype != CTB_F16 && dtype != CTB_BF16 && dtype != CTB_F32)
+    return set_error(CTB_ERR_DTYPE, n + ": logits must be Float16, BFloat16 or Float32");
+  if (T < 0) return set_error(CTB_ERR_SHAPE, n + ": negative number of rows");
+  if (E < 1 || E > ROUTE_MAX_EXPERTS) return set_error(CTB_ERR_SHAPE, n + ": 1 to 256 experts");
+  if (topk < 1 || topk > ROUTE_MAX_TOPK || topk > E)
+    return set_error(CTB_ERR_SHAPE, n + ": topk must be 1 to min(experts, 32)");
+  if (ldx < E) return set_error(CTB_ERR_LAYOUT, n + ": row stride smaller than the row");
+  if (score != CTB_SCORE_SOFTMAX && score != CTB_SCORE_SIGMOID)
+    return set_error(CTB_ERR_ARG, n + ": unknown score");
+  return CTB_OK;
+}
+
+}  // namespace
+}  // namespace ctb
+
+using namespace ctb;
+
+extern "C" int ctb_moe_route(int32_t dtype, const void* logits, const float* bias, float* weights,
+                             int32_t* ids, int32_t T, int32_t E, int32_t topk, int64_t ldx,
+                             int32_t score, int32_t groups, int32_t topk_groups,
+                             int32_t group_top, int32_t renorm, float scale, void* stream) {
+  clear_error();
+  if (int rc = route_check("moe_route", dtype, T, E, topk, ldx, score)) return rc;
+  if (groups < 1 || groups > 32 || E % groups != 0)
+    return set_error(CTB_ERR_SHAPE, "moe_route: 1 to 32 groups that divide the experts");
+  if (topk_groups < 1 || topk_groups > groups)
+    return set_error(CTB_ERR_SHAPE, "moe_route: topk_groups must be 1 to groups");
+  if (group_top != 1 && group_top != 2)
+    return set_error(CTB_ERR_ARG, "moe_route: group_top must be 1 or 2");
+  if (topk > topk_groups * (E / groups))
+    return set_error(CTB_ERR_SHAPE, "moe_route: topk exceeds the experts of topk_groups groups");
+  if (T == 0) return CTB_OK;
+  if (!logits || !weights || !ids) return set_error(CTB_ERR_ARG, "moe_route: NULL pointer");
+  DeviceProps pr;
+  if (int rc = current_props(&pr)) return rc;
+  RouteArgs a;
+  a.bias = bias;
+  a.weights = weights;
+  a.ids = ids;
+  a.T = T;
+  a.E = E;
+  a.topk = topk;
+  a.ldx = ldx;
+  a.sigmoid = score == CTB_SCORE_SIGMOID;
+  a.groups = groups;
+  a.topk_groups = topk_groups;
+  a.group_top = group_top;
+  a.renorm = renorm != 0;
+  a.scale = scale;
+  auto st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case CTB_F16: return route_dispatch((const __half*)logits, a, st);
+    case CTB_BF16: return route_dispatch((const __nv_bfloat16*)logits, a, st);
+    default: return route_dispatch((const float*)logits, a, st);
+  }
+}
+
+extern "C" int ctb_moe_route_bwd(int32_t dtype, const float* dweights, const void* logits,
+                                 const int32_t* ids, void* dlogits, int32_t T, int32_t E,
+                                 int32_t topk, int64_t ldx, int64_t lddx, int32_t score,
+                                 int32_t renorm, float scale, void* stream) {
+  clear_error();
+  if (int rc = route_check("moe_route_bwd", dtype, T, E, topk, ldx, score)) return rc;
+  if (lddx < E)
+    return set_error(CTB_ERR_LAYOUT, "moe_route_bwd: row stride smaller than the row");
+  if (T == 0) return CTB_OK;
+  if (!dweights || !logits || !ids || !dlogits)
+    return set_error(CTB_ERR_ARG, "moe_route_bwd: NULL pointer");
+  DeviceProps pr;
+  if (int rc = current_props(&pr)) return rc;
+  RouteBwdArgs a;
+  a.dweights = dweights;
+  a.ids = ids;
+  a.T = T;
+  a.E = E;
+  a.topk = topk;
+  a.ldx = ldx;
+  a.lddx = lddx;
+  a.sigmoid = score == CTB_SCORE_SIGMOID;
+  a.renorm = renorm != 0;
+  a.scale = scale;
+  auto st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case CTB_F16:
+      return route_bwd_dispatch((const __half*)logits, (__half*)dlogits, a, st);
+    case CTB_BF16:
+      return route_bwd_dispatch((const __nv_bfloat16*)logits, (__nv_bfloat16*)dlogits, a, st);
+    default: return route_bwd_dispatch((const float*)logits, (float*)dlogits, a, st);
+  }
+}

@@ -13,6 +13,7 @@ DEFAULT_LIB = os.path.join(HERE, "libcutile_b200.so")
 
 CTB_MAX_DIMS = 5
 CTB_F16, CTB_BF16, CTB_F32, CTB_F64, CTB_I32 = 1, 2, 3, 4, 5
+CTB_SCORE_SOFTMAX, CTB_SCORE_SIGMOID = 0, 1
 
 STATUS = {
     0: "CTB_OK",
@@ -95,6 +96,12 @@ SIGNATURES = {
     "ctb_vadd_host": [_I32, _P, _P, _P, _I64, _P, _I64, _P],
     "ctb_moe_gemm_f16": [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
                          _I32, _I64, _I64, _I64, _P, _I64, _P],
+    "ctb_moe_route": [_I32, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I32, _I32, _I32, _I32, _I32,
+                      _F, _P],
+    "ctb_moe_route_bwd": [_I32, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I32, _I32, _F, _P],
+    "ctb_moe_combine": [_I32, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I64, _I64, _I64, _P],
+    "ctb_moe_combine_bwd": [_I32, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I64, _I64,
+                            _I64, _P],
     "ctb_fill_uniform": [_P, _I32, _I64, _U64, _U64, _D, _D, _P],
     "ctb_fill_normal": [_P, _I32, _I64, _U64, _U64, _D, _D, _P],
     "ctb_selftest_wait_timeout": [_I64, _P, _P],

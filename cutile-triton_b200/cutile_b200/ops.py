@@ -283,6 +283,200 @@ def moe_gemm(A, B, sorted_ids, expert_ids, ntp, topk, weights=None, out=None, wo
     return out
 
 
+# ---- mixture-of-experts layer: routing and combine ------------------------------
+_SCORES = {"softmax": _lib.CTB_SCORE_SOFTMAX, "sigmoid": _lib.CTB_SCORE_SIGMOID}
+
+
+def _need(ok, code, msg):
+    if not ok:
+        raise _lib.B200Error(code, msg)
+
+
+def _need_matrix(t, rows, cols, dtype, device, what):
+    """A (rows, cols) CUDA matrix of `dtype` on `device` with contiguous rows."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise _lib.B200Error(-1, f"{what}: expected a CUDA tensor")
+    if t.device != device:
+        raise _lib.B200Error(-1, f"{what}: on {t.device}, the other tensors are on {device}")
+    if t.dtype != dtype:
+        raise _lib.B200Error(-2, f"{what}: expected {dtype}, got {t.dtype}")
+    if t.shape != (rows, cols):
+        raise _lib.B200Error(-3, f"{what}: expected shape ({rows}, {cols}), got {tuple(t.shape)}")
+    if cols > 1 and t.stride(1) != 1:
+        raise _lib.B200Error(-4, f"{what}: rows must be contiguous")
+    return t
+
+
+def _need_packed(t, shape, dtype, device, what):
+    """A contiguous CUDA tensor of exactly this shape and dtype."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise _lib.B200Error(-1, f"{what}: expected a CUDA tensor")
+    if t.device != device:
+        raise _lib.B200Error(-1, f"{what}: on {t.device}, the other tensors are on {device}")
+    if t.dtype != dtype:
+        raise _lib.B200Error(-2, f"{what}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise _lib.B200Error(-3, f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise _lib.B200Error(-4, f"{what}: must be contiguous")
+    return t
+
+
+def _ld(t):
+    """Row stride for the C ABI. A single row has none that matters (torch
+    gives any number for it): its length does."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call_on(device, name, *args):
+    """One library call on the current stream of `device`, which need not be
+    the current device."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def moe_route(logits, topk, score="softmax", bias=None, groups=1, topk_groups=None, group_top=2,
+              renorm=True, scale=1.0, weights=None, ids=None):
+    """Routes each row of `logits` (T, E) to `topk` experts -> (weights (T, topk)
+    float32, ids (T, topk) int32), the `topk_ids` of :func:`moe_align` and the
+    `weights` of :func:`moe_gemm` or :func:`moe_combine`.
+
+    The scores s are the row's softmax or sigmoid; c = s + `bias` (E floats)
+    decides the choice only. Of `groups` equal runs of experts the
+    `topk_groups` (default: all) with the largest sum of their `group_top`
+    best c are kept, then the `topk` largest c are taken, largest first, ties
+    to the lowest index. The weights are `scale` * s, with `renorm` divided by
+    the sum of the chosen s. An expert with a logit or c of -inf or NaN is not
+    available; places no expert is left for get id -1 and weight 0 (a row of
+    -inf, a padding token, goes to no expert). E <= 256, topk <= 32."""
+    _need_cuda(logits)
+    _need(logits.dim() == 2, -3, "moe_route: logits must be (T, E)")
+    _need(isinstance(topk, int) and topk >= 1, -3, "moe_route: topk must be positive")
+    _need(score in _SCORES, -1, f"moe_route: unknown score {score!r}")
+    _need(logits.dtype in _DT, -2, f"moe_route: unsupported dtype {logits.dtype}")
+    T, E = logits.shape
+    dev = logits.device
+    _need_matrix(logits, T, E, logits.dtype, dev, "moe_route: logits")
+    if bias is not None:
+        _need_packed(bias, (E,), torch.float32, dev, "moe_route: bias")
+    if weights is None:
+        weights = torch.empty((T, topk), dtype=torch.float32, device=dev)
+    else:
+        _need_packed(weights, (T, topk), torch.float32, dev, "moe_route: weights")
+    if ids is None:
+        ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
+    else:
+        _need_packed(ids, (T, topk), torch.int32, dev, "moe_route: ids")
+    _call_on(dev, "ctb_moe_route", _DT[logits.dtype], logits.data_ptr(), _ptr(bias),
+             weights.data_ptr(), ids.data_ptr(), T, E, topk, _ld(logits), _SCORES[score], groups,
+             groups if topk_groups is None else topk_groups, group_top, 1 if renorm else 0, scale)
+    return weights, ids
+
+
+def moe_route_bwd(dweights, logits, ids, score="softmax", renorm=True, scale=1.0, dlogits=None):
+    """Gradient of :func:`moe_route`'s weights: dlogits (T, E, dtype of the
+    logits) from dweights (T, topk) and the ids of the forward call. The
+    choice and its bias have no gradient."""
+    _need_cuda(dweights, logits, ids)
+    _need(logits.dim() == 2 and ids.dim() == 2, -3,
+          "moe_route_bwd: logits must be (T, E), ids (T, topk)")
+    _need(score in _SCORES, -1, f"moe_route_bwd: unknown score {score!r}")
+    _need(logits.dtype in _DT, -2, f"moe_route_bwd: unsupported dtype {logits.dtype}")
+    T, E = logits.shape
+    topk = ids.shape[1]
+    dev = logits.device
+    _need_matrix(logits, T, E, logits.dtype, dev, "moe_route_bwd: logits")
+    _need_packed(ids, (T, topk), torch.int32, dev, "moe_route_bwd: ids")
+    _need_packed(dweights, (T, topk), torch.float32, dev, "moe_route_bwd: dweights")
+    if dlogits is None:
+        dlogits = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    else:
+        _need_matrix(dlogits, T, E, logits.dtype, dev, "moe_route_bwd: dlogits")
+    _call_on(dev, "ctb_moe_route_bwd", _DT[logits.dtype], dweights.data_ptr(), logits.data_ptr(),
+             ids.data_ptr(), dlogits.data_ptr(), T, E, topk, _ld(logits), _ld(dlogits),
+             _SCORES[score], 1 if renorm else 0, scale)
+    return dlogits
+
+
+def _combine_args(k, rows, topk, weights, ids, num_experts, dev):
+    _need(isinstance(topk, int) and topk >= 1 and rows % topk == 0, -3,
+          f"{k}: y must have T * topk rows")
+    T = rows // topk
+    if weights is not None:
+        _need_packed(weights, (T, topk), torch.float32, dev, f"{k}: weights")
+    if ids is not None:
+        _need_packed(ids, (T, topk), torch.int32, dev, f"{k}: ids")
+        _need(num_experts is not None, -1, f"{k}: ids need num_experts")
+    return T, int(num_experts) if ids is not None else 0
+
+
+def moe_combine(y, topk, weights=None, ids=None, num_experts=None, residual=None, out=None):
+    """One row per token from the experts' rows: out[t] = residual[t] +
+    sum_j weights[t, j] * y[t * topk + j], summed in float32 and rounded once.
+    y: (T * topk, N) float16 or bfloat16, as :func:`moe_gemm` writes it;
+    weights: (T, topk) float32, None where the GEMM has applied them. With
+    `ids` (T, topk) int32 and `num_experts`, slots with an id outside
+    [0, num_experts) are skipped: no expert wrote their rows, which are not
+    read. `out` may be `residual`."""
+    _need_cuda(y)
+    _need(y.dim() == 2, -3, "moe_combine: y must be (T * topk, N)")
+    _need(y.dtype in _DT, -2, f"moe_combine: unsupported dtype {y.dtype}")
+    rows, N = y.shape
+    dev = y.device
+    _need_matrix(y, rows, N, y.dtype, dev, "moe_combine: y")
+    T, E = _combine_args("moe_combine", rows, topk, weights, ids, num_experts, dev)
+    if residual is not None:
+        _need_matrix(residual, T, N, y.dtype, dev, "moe_combine: residual")
+    if out is None:
+        out = torch.empty((T, N), dtype=y.dtype, device=dev)
+    else:
+        _need_matrix(out, T, N, y.dtype, dev, "moe_combine: out")
+    _call_on(dev, "ctb_moe_combine", _DT[y.dtype], y.data_ptr(), _ptr(weights), _ptr(ids),
+             _ptr(residual), out.data_ptr(), T, topk, N, E, _ld(y),
+             0 if residual is None else _ld(residual), _ld(out))
+    return out
+
+
+def moe_combine_bwd(dout, y, topk, weights=None, ids=None, num_experts=None, dy=None,
+                    dweights=None):
+    """Gradients of :func:`moe_combine` -> (dy (T * topk, N), dweights (T, topk)
+    float32, None without weights). Skipped slots get zeros. The gradient of
+    the residual is `dout`. Without weights `y` is not used and may be None."""
+    _need_cuda(dout)
+    _need(dout.dim() == 2, -3, "moe_combine_bwd: dout must be (T, N)")
+    _need(dout.dtype in _DT, -2, f"moe_combine_bwd: unsupported dtype {dout.dtype}")
+    T, N = dout.shape
+    dev = dout.device
+    _need(isinstance(topk, int) and topk >= 1, -3, "moe_combine_bwd: topk must be positive")
+    rows = T * topk
+    _need_matrix(dout, T, N, dout.dtype, dev, "moe_combine_bwd: dout")
+    T, E = _combine_args("moe_combine_bwd", rows, topk, weights, ids, num_experts, dev)
+    if weights is None:
+        _need(dweights is None, -1, "moe_combine_bwd: dweights without weights")
+        y = None
+    else:
+        _need_matrix(y, rows, N, dout.dtype, dev, "moe_combine_bwd: y")
+        if dweights is None:
+            dweights = torch.empty((T, topk), dtype=torch.float32, device=dev)
+        else:
+            _need_packed(dweights, (T, topk), torch.float32, dev, "moe_combine_bwd: dweights")
+    if dy is None:
+        dy = torch.empty((rows, N), dtype=dout.dtype, device=dev)
+    else:
+        _need_matrix(dy, rows, N, dout.dtype, dev, "moe_combine_bwd: dy")
+    _call_on(dev, "ctb_moe_combine_bwd", _DT[dout.dtype], dout.data_ptr(), _ptr(y), _ptr(weights),
+             _ptr(ids), dy.data_ptr(), _ptr(dweights), T, topk, N, E, _ld(dout),
+             0 if y is None else _ld(y), _ld(dy))
+    return dy, dweights
+
+
 # ---- host-buffer calls (three-stream chunk pipeline inside the library) -------
 _host_ws = {}
 

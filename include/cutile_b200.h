@@ -294,6 +294,64 @@ int ctb_moe_gemm_f16(const void* A, const void* B, void* C,
                      int32_t topk, int32_t block_m, int64_t lda, int64_t ldb, int64_t ldc,
                      void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- mixture-of-experts layer: routing and combine -------------------------- */
+
+/* Scores of ctb_moe_route. */
+typedef enum { CTB_SCORE_SOFTMAX = 0, CTB_SCORE_SIGMOID = 1 } ctb_score;
+
+/* Routing of T tokens to topk of E experts (the step before ctb_moe_align_i32
+ * and ctb_moe_gemm_f16; no counterpart in the reference, whose moe example
+ * takes topk_ids as given). logits: T rows of E contiguous elements, row
+ * stride ldx, dtype F16, BF16 or F32. With s = softmax(row) or sigmoid(row)
+ * and c = s + bias (bias: E floats or NULL; it steers the choice only):
+ *   - of `groups` equal runs of experts (1..32, dividing E) the topk_groups
+ *     with the largest sum of their group_top (1 or 2) best c are kept;
+ *   - the topk experts with the largest c are chosen, largest first, ties to
+ *     the lowest index (groups too);
+ *   - weights[t, j] = scale * s of choice j, divided by the sum of the chosen
+ *     s where renorm is not 0.
+ * An expert whose logit or c is -inf or NaN is not available; a place that no
+ * expert is left for gets id -1 (which ctb_moe_align_i32 does not list) and
+ * weight 0, so a row of -inf routes a padding token nowhere. A logit of +inf
+ * gives NaN weights under softmax, as the formula does. The choice is that of
+ * exact arithmetic, also where c differs by less than Float32 resolves.
+ * weights and ids: T x topk, contiguous. E <= 256, topk <= 32. */
+int ctb_moe_route(int32_t dtype, const void* logits, const float* bias, float* weights,
+                  int32_t* ids, int32_t T, int32_t E, int32_t topk, int64_t ldx, int32_t score,
+                  int32_t groups, int32_t topk_groups, int32_t group_top, int32_t renorm,
+                  float scale, void* stream);
+
+/* Gradient of ctb_moe_route's weights with respect to the logits: dlogits
+ * (T x E, row stride lddx, dtype of the logits) from dweights (T x topk) and
+ * the ids that the forward call gave; `score`, `renorm` and `scale` as there.
+ * Places with an id outside [0, E) or a logit of -inf or NaN give nothing. */
+int ctb_moe_route_bwd(int32_t dtype, const float* dweights, const void* logits,
+                      const int32_t* ids, void* dlogits, int32_t T, int32_t E, int32_t topk,
+                      int64_t ldx, int64_t lddx, int32_t score, int32_t renorm, float scale,
+                      void* stream);
+
+/* The experts' rows back to one row per token (the step after the last
+ * ctb_moe_gemm_f16): out[t, :] = residual[t, :] + sum_j w[t, j] * y[t * topk + j, :],
+ * summed in Float32 in the order of j, rounded once. y: T * topk rows of N
+ * contiguous elements, dtype F16 or BF16, row stride ldy; weights: T x topk
+ * floats or NULL (all 1: ctb_moe_gemm_f16 may have applied them); residual:
+ * row stride ldr, or NULL; out: row stride ldo, may be the residual itself.
+ * ids: T x topk or NULL; a slot whose id is outside [0, E) was given to no
+ * expert: its row of y is not read and its weight not used. */
+int ctb_moe_combine(int32_t dtype, const void* y, const float* weights, const int32_t* ids,
+                    const void* residual, void* out, int32_t T, int32_t topk, int32_t N,
+                    int32_t E, int64_t ldy, int64_t ldr, int64_t ldo, void* stream);
+
+/* Gradients of ctb_moe_combine: dy[t * topk + j, :] = w[t, j] * dout[t, :] and
+ * dweights[t, j] = sum_n dout[t, n] * y[t * topk + j, n] (Float32). Slots with
+ * an id outside [0, E) get zeros in both, their rows of y are not read. With
+ * weights NULL, y and dweights are not used and may be NULL. The gradient of
+ * the residual is dout itself. */
+int ctb_moe_combine_bwd(int32_t dtype, const void* dout, const void* y, const float* weights,
+                        const int32_t* ids, void* dy, float* dweights, int32_t T, int32_t topk,
+                        int32_t N, int32_t E, int64_t lddo, int64_t ldy, int64_t lddy,
+                        void* stream);
+
 /* ---- seeded synthetic inputs (bench / test plumbing, not a cuTile op) ---- */
 
 /* Counter-based SplitMix64 stream: element i uses counter offset + i.

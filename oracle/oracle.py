@@ -252,6 +252,119 @@ def moe(A, B, sorted_ids, expert_ids, num_post_padded, topk, weights=None, block
     return C
 
 
+def moe_route(x, topk, score="softmax", bias=None, groups=1, topk_groups=None, group_top=2,
+              renorm=True, scale=1.0):
+    """Float64 routing, row by row: (weights (T, topk), ids (T, topk)). Scores
+    are the row's softmax or sigmoid; score + bias decides the choice; the
+    topk_groups groups with the largest sum of their group_top best are kept;
+    ties go to the lowest index; experts at -inf or NaN are never chosen and
+    places left over get id -1, weight 0. Without a bias experts rank by
+    their logits, in which the scores rise."""
+    x = np.asarray(x, np.float64)
+    x = np.where(np.isnan(x), -np.inf, x)
+    T, E = x.shape
+    topk_groups = groups if topk_groups is None else topk_groups
+    W, I = np.zeros((T, topk)), np.full((T, topk), -1, np.int32)
+    for t in range(T):
+        row = x[t]
+        live = row > -np.inf
+        if not live.any():
+            continue
+        top = row.max()
+        with np.errstate(over="ignore", invalid="ignore"):
+            if score == "softmax":
+                p = np.exp(row - top)
+                s = p / p.sum()
+            else:
+                s = 1 / (1 + np.exp(-row))
+        c = s if bias is None else s + np.asarray(bias, np.float64)
+        live &= c > -np.inf
+        size = E // groups
+        if topk_groups < groups:
+            sums = []
+            for g in range(groups):
+                best = sorted((c[e] for e in range(g * size, (g + 1) * size) if live[e]), reverse=True)
+                sums.append(sum(best[:group_top]) if best else -np.inf)
+            kept = sorted(range(groups), key=lambda g: (-sums[g], g))[:topk_groups]
+            for g in range(groups):
+                if g not in kept:
+                    live[g * size:(g + 1) * size] = False
+        rank = row if bias is None else c
+        order = sorted((e for e in range(E) if live[e]), key=lambda e: (-rank[e], e))[:topk]
+        if not order:
+            continue
+        I[t, :len(order)] = order
+        if renorm:
+            r = row[order]
+            if score == "softmax":
+                v = np.exp(r - r.max())
+            else:  # log sigmoid, shifted by its largest value
+                ls = np.where(r < 0, r, 0) - np.log1p(np.exp(-np.abs(r)))
+                v = np.exp(ls - ls.max())
+            W[t, :len(order)] = scale * v / v.sum()
+        else:
+            W[t, :len(order)] = scale * s[order]
+    return W, I
+
+
+def moe_route_bwd(dw, x, ids, score="softmax", renorm=True, scale=1.0):
+    """Float64 gradient of moe_route's weights for fixed ids, by the Jacobian of
+    each row: dx[e] = sum_j dw[j] * dweight[j]/dx[e]."""
+    x = np.asarray(x, np.float64)
+    x = np.where(np.isnan(x), -np.inf, x)
+    dw = np.asarray(dw, np.float64)
+    dx = np.zeros_like(x)
+    for t in range(x.shape[0]):
+        js = [j for j, e in enumerate(ids[t]) if 0 <= e < x.shape[1] and x[t, e] > -np.inf]
+        if not js:
+            continue
+        es = [int(ids[t, j]) for j in js]
+        if score == "softmax":
+            p = np.exp(x[t] - x[t].max())
+            p /= p.sum()
+            J = -np.outer(p[es], p)  # ds[j] / dx[e]
+            for r, e in enumerate(es):
+                J[r, e] += p[e]
+            s = p[es]
+        else:
+            s = 1 / (1 + np.exp(-x[t, es]))
+            J = np.zeros((len(es), x.shape[1]))
+            for r, e in enumerate(es):
+                J[r, e] = s[r] / (1 + np.exp(x[t, e]))
+        if renorm:
+            J = J / s.sum() - np.outer(s, J.sum(0)) / s.sum() ** 2
+        dx[t] = scale * dw[t, js] @ J
+    return dx
+
+
+def moe_combine(y, topk, weights=None, ids=None, num_experts=0, residual=None):
+    """Float64 out[t] = residual[t] + sum_j w[t, j] * y[t * topk + j], slots with
+    an id outside [0, num_experts) left out."""
+    y = np.asarray(y, np.float64)
+    T = y.shape[0] // topk
+    out = np.zeros((T, y.shape[1])) if residual is None else np.array(residual, np.float64)
+    for t in range(T):
+        for j in range(topk):
+            if ids is None or 0 <= ids[t, j] < num_experts:
+                out[t] += (1.0 if weights is None else float(weights[t, j])) * y[t * topk + j]
+    return out
+
+
+def moe_combine_bwd(dout, y, topk, weights=None, ids=None, num_experts=0):
+    """Float64 (dy, dweights) of moe_combine; dweights None without weights."""
+    dout = np.asarray(dout, np.float64)
+    T, N = dout.shape
+    dy = np.zeros((T * topk, N))
+    dw = None if weights is None else np.zeros((T, topk))
+    for t in range(T):
+        for j in range(topk):
+            if ids is None or 0 <= ids[t, j] < num_experts:
+                dy[t * topk + j] = (1.0 if weights is None else float(weights[t, j])) * dout[t]
+                if weights is not None:
+                    dw[t, j] = dout[t] @ np.asarray(y[t * topk + j], np.float64)
+    return dy, dw
+
+
 # ---- float-accumulating variants: the timed CPU baseline ------------------------
 def vadd_f32_into(a, b, c):
     lib().oracle_vadd_f32(_p(a), _p(b), _p(c), a.size)
