@@ -1,0 +1,299 @@
+// The dense layer: a matrix product with bias, activation and residual in its
+// epilogue, and its gradients (ctb_dense_fwd, ctb_dense_bwd).
+//
+//   Z = A B .+ b,  C = act.(Z) .+ R               (Julia, column-major)
+//   dZ = dC .* act'(Z),  db = sum(dZ; dims = 2),  dA = dZ B',  dB = A' dZ
+//
+// dZ is rounded to the operands' 16 bits: it is an operand of two tensor-core
+// products. db is summed from the unrounded values, in Float32.
+#include "dense.cuh"
+
+#include <algorithm>
+
+namespace ctb {
+namespace dense {
+namespace {
+
+// ---- general product: any size, stride and alignment, on the CUDA cores ---------------
+// 256 threads; each computes a 4 x 4 block of a 64 x 64 tile of D.
+constexpr int SG = 64, SG_K = 16;
+
+template <typename T>
+__global__ void __launch_bounds__(256) product_simt_kernel(const Product p) {
+  __shared__ float Ps[SG_K][SG + 1];
+  __shared__ float Qs[SG_K][SG + 1];
+  const T* P = static_cast<const T*>(p.P);
+  const T* Q = static_cast<const T*>(p.Q);
+  const int64_t prs = p.p_mn ? 1 : p.ldp, pks = p.p_mn ? p.ldp : 1;
+  const int64_t qcs = p.q_mn ? 1 : p.ldq, qks = p.q_mn ? p.ldq : 1;
+  const int c0 = blockIdx.x * SG;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  for (int64_t r0 = (int64_t)blockIdx.y * SG; r0 < p.rows; r0 += (int64_t)gridDim.y * SG) {
+    float acc[4][4] = {};
+    for (int k0 = 0; k0 < p.depth; k0 += SG_K) {
+      for (int i = threadIdx.x; i < SG * SG_K; i += 256) {
+        const int a = p.p_mn ? i % SG : i / SG_K, ka = p.p_mn ? i / SG : i % SG_K;
+        Ps[ka][a] = r0 + a < p.rows && k0 + ka < p.depth
+                        ? to_f32(P[(r0 + a) * prs + (k0 + ka) * pks]) : 0.f;
+        const int b = p.q_mn ? i % SG : i / SG_K, kb = p.q_mn ? i / SG : i % SG_K;
+        Qs[kb][b] = c0 + b < p.cols && k0 + kb < p.depth
+                        ? to_f32(Q[(c0 + b) * qcs + (k0 + kb) * qks]) : 0.f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < SG_K; ++k) {
+        float a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = Ps[k][ty + 16 * i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = Qs[k][tx + 16 * j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t r = r0 + ty + 16 * i;
+        const int c = c0 + tx + 16 * j;
+        if (r >= p.rows || c >= p.cols) continue;
+        float z = acc[i][j];
+        if (p.bias)
+          z += p.bias_f32 ? static_cast<const float*>(p.bias)[c]
+                          : to_f32(static_cast<const T*>(p.bias)[c]);
+        if (p.Z) from_f32(static_cast<T*>(p.Z) + r * p.ldz + c, z);
+        float v = activate_any(z, p.act);
+        if (p.R) v += to_f32(static_cast<const T*>(p.R)[r * p.ldr + c]);
+        from_f32(static_cast<T*>(p.D) + r * p.ldd + c, v);
+      }
+  }
+}
+
+template <typename T>
+int product(const Product& p, cudaStream_t st) {
+  const dim3 grid((p.cols + SG - 1) / SG, std::min((p.rows + SG - 1) / SG, 65535));
+  product_simt_kernel<T><<<grid, 256, 0, st>>>(p);
+  return launch_status("product_simt_kernel");
+}
+
+// ---- dZ = dC .* act'(Z) and its column sums ---------------------------------------------
+// A CTA takes SUM_COLS columns and a span of rows; spans are summed afterwards
+// in order, so the result does not depend on the schedule.
+constexpr int SUM_COLS = 64, SUM_THREADS = 256, SUM_LANES = SUM_THREADS / SUM_COLS;
+
+template <typename T>
+__global__ void __launch_bounds__(SUM_THREADS)
+    slope_kernel(const T* __restrict__ dC, const T* __restrict__ Z, T* __restrict__ dZ,
+                 float* __restrict__ partial, int N, int M, int64_t lddc, int64_t ldz,
+                 int64_t lddz, int act, int span) {
+  __shared__ float red[SUM_LANES][SUM_COLS];
+  const int cl = threadIdx.x % SUM_COLS, rl = threadIdx.x / SUM_COLS;
+  const int c = blockIdx.x * SUM_COLS + cl;
+  const int64_t n0 = (int64_t)blockIdx.y * span, n1 = min((int64_t)N, n0 + span);
+  float sum = 0.f;
+  if (c < M)
+    for (int64_t n = n0 + rl; n < n1; n += SUM_LANES) {
+      float d = to_f32(dC[n * lddc + c]);
+      if (Z) {
+        const float z = to_f32(Z[n * ldz + c]);
+        switch (act) {
+          case CTB_ACT_RELU: d *= activate_slope<CTB_ACT_RELU>(z); break;
+          case CTB_ACT_GELU: d *= activate_slope<CTB_ACT_GELU>(z); break;
+          case CTB_ACT_GELU_TANH: d *= activate_slope<CTB_ACT_GELU_TANH>(z); break;
+          default: d *= activate_slope<CTB_ACT_SILU>(z); break;
+        }
+      }
+      if (dZ) from_f32(dZ + n * lddz + c, d);
+      sum += d;
+    }
+  red[rl][cl] = sum;
+  __syncthreads();
+  if (partial && rl == 0 && c < M) {
+    for (int i = 1; i < SUM_LANES; ++i) sum += red[i][cl];
+    partial[(int64_t)blockIdx.y * M + c] = sum;
+  }
+}
+
+__global__ void fold_kernel(const float* __restrict__ partial, float* __restrict__ out, int M,
+                            int spans) {
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= M) return;
+  float s = 0.f;
+  for (int i = 0; i < spans; ++i) s += partial[(int64_t)i * M + c];
+  out[c] = s;
+}
+
+constexpr int MAX_SPANS = 64;
+int spans_of(int N) { return std::max(1, std::min(MAX_SPANS, (N + 63) / 64)); }
+
+int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+template <typename T>
+int dense_bwd(const T* dC, const T* A, const T* B, const T* Z, T* dA, T* dB, float* dbias, int M,
+              int N, int K, int64_t lddc, int64_t lda, int64_t ldb, int64_t ldz, int64_t ldda,
+              int64_t lddb, int act, uint8_t* ws, cudaStream_t st) {
+  const T* dZ = dC;
+  int64_t lddz = lddc;
+  if (act != CTB_ACT_NONE || dbias) {
+    const int spans = spans_of(N);
+    float* partial = reinterpret_cast<float*>(ws);
+    T* dz = nullptr;
+    if (act != CTB_ACT_NONE) {
+      lddz = round8(M);
+      dz = reinterpret_cast<T*>(ws + (dbias ? round256(4ll * MAX_SPANS * M) : 0));
+      dZ = dz;
+    }
+    if (M > 0) {
+      const dim3 grid((M + SUM_COLS - 1) / SUM_COLS, spans);
+      slope_kernel<T><<<grid, SUM_THREADS, 0, st>>>(
+          dC, act != CTB_ACT_NONE ? Z : nullptr, dz, dbias ? (spans > 1 ? partial : dbias) : nullptr,
+          N, M, lddc, ldz, lddz, act, (N + spans - 1) / spans);
+      if (int rc = launch_status("slope_kernel")) return rc;
+      if (dbias && spans > 1) {
+        fold_kernel<<<(M + 255) / 256, 256, 0, st>>>(partial, dbias, M, spans);
+        if (int rc = launch_status("fold_kernel")) return rc;
+      }
+    }
+  }
+  if (dB && N > 0 && K > 0) {
+    Product p = {};
+    p.P = dZ;
+    p.ldp = lddz;
+    p.Q = A;
+    p.ldq = lda;
+    p.D = dB;
+    p.ldd = lddb;
+    p.rows = N;
+    p.cols = K;
+    p.depth = M;
+    if (int rc = product<T>(p, st)) return rc;
+  }
+  if (dA && M > 0 && K > 0) {
+    Product p = {};
+    p.P = B;
+    p.ldp = ldb;
+    p.p_mn = true;
+    p.Q = dZ;
+    p.ldq = lddz;
+    p.q_mn = true;
+    p.D = dA;
+    p.ldd = ldda;
+    p.rows = K;
+    p.cols = M;
+    p.depth = N;
+    if (int rc = product<T>(p, st)) return rc;
+  }
+  return CTB_OK;
+}
+
+int dense_check(const char* k, int dtype, int M, int N, int K, int act) {
+  const std::string n(k);
+  if (dtype != CTB_F16 && dtype != CTB_BF16)
+    return set_error(CTB_ERR_DTYPE, n + ": matrices must be Float16 or BFloat16");
+  if (M < 0 || N < 0 || K < 0) return set_error(CTB_ERR_SHAPE, n + ": negative size");
+  if (act < CTB_ACT_NONE || act > CTB_ACT_SILU)
+    return set_error(CTB_ERR_ARG, n + ": unknown activation");
+  return CTB_OK;
+}
+
+}  // namespace
+}  // namespace dense
+}  // namespace ctb
+
+using namespace ctb;
+
+extern "C" int64_t ctb_dense_fwd_workspace_bytes(const void* A, const void* B, int32_t M, int32_t N,
+                                                 int32_t K, int64_t lda, int64_t ldb) {
+  (void)A, (void)B, (void)M, (void)N, (void)K, (void)lda, (void)ldb;
+  return 0;
+}
+
+extern "C" int64_t ctb_dense_bwd_workspace_bytes(const void* dC, const void* A, const void* B,
+                                                 int32_t M, int32_t N, int32_t K, int64_t lddc,
+                                                 int64_t lda, int64_t ldb, int32_t act,
+                                                 int32_t need_dbias) {
+  (void)dC, (void)A, (void)B, (void)K, (void)lddc, (void)lda, (void)ldb;
+  if (M < 0 || N < 0 || K < 0) return -1;
+  int64_t b = need_dbias ? dense::round256(4ll * dense::MAX_SPANS * M) : 0;
+  if (act != CTB_ACT_NONE) b += dense::round256(2ll * N * dense::round8(M));
+  return b;
+}
+
+extern "C" int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const void* bias,
+                             int32_t bias_dtype, const void* R, void* Z, void* C, int32_t M,
+                             int32_t N, int32_t K, int64_t lda, int64_t ldb, int64_t ldr,
+                             int64_t ldz, int64_t ldc, int32_t act, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = dense::dense_check("dense", dtype, M, N, K, act)) return rc;
+  if (bias && bias_dtype != dtype && bias_dtype != CTB_F32)
+    return set_error(CTB_ERR_DTYPE, "dense: the bias must be Float32 or of the matrices' type");
+  if (lda < M || ldb < K || ldc < M || (R && ldr < M) || (Z && ldz < M))
+    return set_error(CTB_ERR_LAYOUT, "dense: leading dimension smaller than the column length");
+  if (M == 0 || N == 0) return CTB_OK;
+  if (!C || (K > 0 && (!A || !B))) return set_error(CTB_ERR_ARG, "dense: NULL pointer");
+  const int64_t need = ctb_dense_fwd_workspace_bytes(A, B, M, N, K, lda, ldb);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return set_error(CTB_ERR_ARG, "dense: the workspace needs " + std::to_string(need) +
+                                      " bytes, 16-byte aligned");
+  DeviceProps pr;
+  if (int rc = current_props(&pr)) return rc;
+  dense::Product p = {};
+  p.P = B;
+  p.ldp = ldb;
+  p.Q = A;
+  p.ldq = lda;
+  p.q_mn = true;
+  p.D = C;
+  p.ldd = ldc;
+  p.rows = N;
+  p.cols = M;
+  p.depth = K;
+  p.bias = bias;
+  p.bias_f32 = bias_dtype == CTB_F32;
+  p.act = act;
+  p.R = R;
+  p.ldr = ldr;
+  p.Z = Z;
+  p.ldz = ldz;
+  auto st = static_cast<cudaStream_t>(stream);
+  return dtype == CTB_F16 ? dense::product<__half>(p, st) : dense::product<__nv_bfloat16>(p, st);
+}
+
+extern "C" int ctb_dense_bwd(int32_t dtype, const void* dC, const void* A, const void* B,
+                             const void* Z, void* dA, void* dB, float* dbias, int32_t M, int32_t N,
+                             int32_t K, int64_t lddc, int64_t lda, int64_t ldb, int64_t ldz,
+                             int64_t ldda, int64_t lddb, int32_t act, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = dense::dense_check("dense_bwd", dtype, M, N, K, act)) return rc;
+  const bool slope = act != CTB_ACT_NONE;
+  if (lddc < M || (dB && lda < M) || (dA && ldb < K) || (slope && ldz < M) || (dA && ldda < M) ||
+      (dB && lddb < K))
+    return set_error(CTB_ERR_LAYOUT, "dense_bwd: leading dimension smaller than the column length");
+  const bool some = M > 0 && N > 0;
+  if ((some && (!dC || (slope && !Z))) || (some && K > 0 && ((dB && !A) || (dA && !B))))
+    return set_error(CTB_ERR_ARG, "dense_bwd: NULL pointer");
+  const int64_t need = ctb_dense_bwd_workspace_bytes(dC, A, B, M, N, K, lddc, lda, ldb, act,
+                                                     dbias != nullptr);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return set_error(CTB_ERR_ARG, "dense_bwd: the workspace needs " + std::to_string(need) +
+                                      " bytes, 16-byte aligned");
+  DeviceProps pr;
+  if (int rc = current_props(&pr)) return rc;
+  auto st = static_cast<cudaStream_t>(stream);
+  auto* ws = static_cast<uint8_t*>(workspace);
+  if (dtype == CTB_F16)
+    return dense::dense_bwd<__half>((const __half*)dC, (const __half*)A, (const __half*)B,
+                                    (const __half*)Z, (__half*)dA, (__half*)dB, dbias, M, N, K,
+                                    lddc, lda, ldb, ldz, ldda, lddb, act, ws, st);
+  using bf = __nv_bfloat16;
+  return dense::dense_bwd<bf>((const bf*)dC, (const bf*)A, (const bf*)B, (const bf*)Z, (bf*)dA,
+                              (bf*)dB, dbias, M, N, K, lddc, lda, ldb, ldz, ldda, lddb, act, ws,
+                              st);
+}

@@ -131,10 +131,13 @@ template <> struct KeyOf<double> { using type = uint64_t; };
 
 template <int LANES>
 __device__ __forceinline__ uint32_t row_max_key(uint32_t v) {
-  if (LANES == 32) return __reduce_max_sync(FULL, v);
+  if constexpr (LANES == 32) {
+    return __reduce_max_sync(FULL, v);
+  } else {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL, v, o));
-  return v;
+    for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(FULL, v, o));
+    return v;
+  }
 }
 template <int LANES>
 __device__ __forceinline__ uint64_t row_max_key(uint64_t v) {

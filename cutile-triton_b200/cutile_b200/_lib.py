@@ -14,6 +14,7 @@ DEFAULT_LIB = os.path.join(HERE, "libcutile_b200.so")
 CTB_MAX_DIMS = 5
 CTB_F16, CTB_BF16, CTB_F32, CTB_F64, CTB_I32 = 1, 2, 3, 4, 5
 CTB_SCORE_SOFTMAX, CTB_SCORE_SIGMOID = 0, 1
+CTB_ACT_NONE, CTB_ACT_RELU, CTB_ACT_GELU, CTB_ACT_GELU_TANH, CTB_ACT_SILU = 0, 1, 2, 3, 4
 
 STATUS = {
     0: "CTB_OK",
@@ -96,6 +97,12 @@ SIGNATURES = {
     "ctb_vadd_host": [_I32, _P, _P, _P, _I64, _P, _I64, _P],
     "ctb_moe_gemm_f16": [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
                          _I32, _I64, _I64, _I64, _P, _I64, _P],
+    "ctb_dense_fwd_workspace_bytes": [_P, _P, _I32, _I32, _I32, _I64, _I64],
+    "ctb_dense_fwd": [_I32, _P, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I64, _I64,
+                      _I64, _I32, _P, _I64, _P],
+    "ctb_dense_bwd_workspace_bytes": [_P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I64, _I32, _I32],
+    "ctb_dense_bwd": [_I32, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I64, _I64,
+                      _I64, _I64, _I32, _P, _I64, _P],
     "ctb_moe_route": [_I32, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I32, _I32, _I32, _I32, _I32,
                       _F, _P],
     "ctb_moe_route_bwd": [_I32, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I32, _I32, _F, _P],
@@ -130,6 +137,8 @@ def load():
         fn.restype = ctypes.c_int
     L.ctb_moe_workspace_bytes.restype = ctypes.c_int64
     L.ctb_host_workspace_bytes.restype = ctypes.c_int64
+    L.ctb_dense_fwd_workspace_bytes.restype = ctypes.c_int64
+    L.ctb_dense_bwd_workspace_bytes.restype = ctypes.c_int64
     L.ctb_last_error.argtypes = []
     L.ctb_last_error.restype = ctypes.c_char_p
     _lib = L

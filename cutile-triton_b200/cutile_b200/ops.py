@@ -283,10 +283,7 @@ def moe_gemm(A, B, sorted_ids, expert_ids, ntp, topk, weights=None, out=None, wo
     return out
 
 
-# ---- mixture-of-experts layer: routing and combine ------------------------------
-_SCORES = {"softmax": _lib.CTB_SCORE_SOFTMAX, "sigmoid": _lib.CTB_SCORE_SIGMOID}
-
-
+# ---- argument checks of the layer calls below ------------------------------------
 def _need(ok, code, msg):
     if not ok:
         raise _lib.B200Error(code, msg)
@@ -340,6 +337,108 @@ def _call_on(device, name, *args):
     else:
         with torch.cuda.device(device):
             _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+# ---- dense layer ------------------------------------------------------------------
+_ACTS = {"none": _lib.CTB_ACT_NONE, "relu": _lib.CTB_ACT_RELU, "gelu": _lib.CTB_ACT_GELU,
+         "gelu_tanh": _lib.CTB_ACT_GELU_TANH, "silu": _lib.CTB_ACT_SILU}
+
+
+def _dense_operands(k, A_t, B_t, act):
+    """Checks the weight (K, M) and the activations (N, K) -> (M, N, K, dtype, device)."""
+    _need_cuda(A_t, B_t)
+    _need(A_t.dim() == 2 and B_t.dim() == 2, -3, f"{k}: A_t must be (K, M), B_t (N, K)")
+    _need(act in _ACTS, -1, f"{k}: unknown activation {act!r}")
+    dt, dev = A_t.dtype, A_t.device
+    _need(dt in (torch.float16, torch.bfloat16), -2, f"{k}: float16 or bfloat16, got {dt}")
+    K, M = A_t.shape
+    N = B_t.shape[0]
+    _need_matrix(A_t, K, M, dt, dev, f"{k}: A_t")
+    _need_matrix(B_t, N, K, dt, dev, f"{k}: B_t")
+    return M, N, K, dt, dev
+
+
+def _workspace(nbytes, device):
+    """Scratch of one call: from torch's allocator, which keeps it to this
+    stream's order and, in a capture, to the graph."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def dense(A_t, B_t, bias=None, act="none", residual=None, out=None, preact=None):
+    """Dense layer on Julia column-major storage, as :func:`matmul`: with A_t
+    (K, M) the weight and B_t (N, K) one row per token, returns (N, M)
+    act(B_t @ A_t + bias) + residual, float16 or bfloat16. `act` is "none",
+    "relu", "gelu", "gelu_tanh" or "silu"; bias (M) is of the matrices' type or
+    float32; `preact` (N, M), when given, receives the value before the
+    activation, which :func:`dense_bwd` needs. `out` may be `residual`. Sums
+    are float32; each output is rounded once."""
+    M, N, K, dt, dev = _dense_operands("dense", A_t, B_t, act)
+    if bias is not None:
+        _need_packed(bias, (M,), bias.dtype if bias.dtype == torch.float32 else dt, dev,
+                     "dense: bias")
+    if residual is not None:
+        _need_matrix(residual, N, M, dt, dev, "dense: residual")
+    if preact is not None:
+        _need_matrix(preact, N, M, dt, dev, "dense: preact")
+    if out is None:
+        out = torch.empty((N, M), dtype=dt, device=dev)
+    else:
+        _need_matrix(out, N, M, dt, dev, "dense: out")
+    lda, ldb = _ld(A_t), _ld(B_t)
+    pa, pb = A_t.data_ptr(), B_t.data_ptr()
+    nws = _lib.load().ctb_dense_fwd_workspace_bytes(pa, pb, M, N, K, lda, ldb)
+    ws = _workspace(nws, dev)
+    _call_on(dev, "ctb_dense_fwd", _DT[dt], pa, pb, _ptr(bias),
+             0 if bias is None else _DT[bias.dtype], _ptr(residual), _ptr(preact), out.data_ptr(),
+             M, N, K, lda, ldb, 0 if residual is None else _ld(residual),
+             0 if preact is None else _ld(preact), _ld(out), _ACTS[act], _ptr(ws), nws)
+    return out
+
+
+def dense_bwd(dC_t, A_t, B_t, act="none", preact=None, dA_t=None, dB_t=None, dbias=None,
+              need_dA=True, need_dB=True, need_dbias=True):
+    """Gradients of :func:`dense` from dC_t (N, M) -> (dA_t (K, M), dB_t (N, K),
+    dbias (M) float32), None for those not needed. `preact` is the forward
+    call's (not used without an activation). The residual's gradient is dC_t."""
+    M, N, K, dt, dev = _dense_operands("dense_bwd", A_t, B_t, act)
+    _need_matrix(dC_t, N, M, dt, dev, "dense_bwd: dC_t")
+    if act != "none":
+        _need(preact is not None, -1, "dense_bwd: an activation's gradient needs preact")
+        _need_matrix(preact, N, M, dt, dev, "dense_bwd: preact")
+    else:
+        preact = None
+    if not need_dA:
+        dA_t = None
+    elif dA_t is None:
+        dA_t = torch.empty((K, M), dtype=dt, device=dev)
+    else:
+        _need_matrix(dA_t, K, M, dt, dev, "dense_bwd: dA_t")
+    if not need_dB:
+        dB_t = None
+    elif dB_t is None:
+        dB_t = torch.empty((N, K), dtype=dt, device=dev)
+    else:
+        _need_matrix(dB_t, N, K, dt, dev, "dense_bwd: dB_t")
+    if not need_dbias:
+        dbias = None
+    elif dbias is None:
+        dbias = torch.empty(M, dtype=torch.float32, device=dev)
+    else:
+        _need_packed(dbias, (M,), torch.float32, dev, "dense_bwd: dbias")
+    lddc, lda, ldb = _ld(dC_t), _ld(A_t), _ld(B_t)
+    pd, pa, pb = dC_t.data_ptr(), A_t.data_ptr(), B_t.data_ptr()
+    nws = _lib.load().ctb_dense_bwd_workspace_bytes(pd, pa, pb, M, N, K, lddc, lda, ldb, _ACTS[act],
+                                                    1 if need_dbias else 0)
+    ws = _workspace(nws, dev)
+    _call_on(dev, "ctb_dense_bwd", _DT[dt], pd, pa, pb, _ptr(preact), _ptr(dA_t), _ptr(dB_t),
+             _ptr(dbias), M, N, K, lddc, lda, ldb, 0 if preact is None else _ld(preact),
+             0 if dA_t is None else _ld(dA_t), 0 if dB_t is None else _ld(dB_t), _ACTS[act],
+             _ptr(ws), nws)
+    return dA_t, dB_t, dbias
+
+
+# ---- mixture-of-experts layer: routing and combine ------------------------------
+_SCORES = {"softmax": _lib.CTB_SCORE_SOFTMAX, "sigmoid": _lib.CTB_SCORE_SIGMOID}
 
 
 def moe_route(logits, topk, score="softmax", bias=None, groups=1, topk_groups=None, group_top=2,

@@ -294,6 +294,52 @@ int ctb_moe_gemm_f16(const void* A, const void* B, void* C,
                      int32_t topk, int32_t block_m, int64_t lda, int64_t ldb, int64_t ldc,
                      void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- dense layer: matrix product with bias, activation and residual ---------- */
+
+/* Activations of the dense layer: none, max(z, 0), z * Phi(z) (Phi the normal
+ * distribution function), its tanh form 0.5 z (1 + tanh(sqrt(2/pi) (z +
+ * 0.044715 z^3))), and z / (1 + exp(-z)). */
+typedef enum {
+  CTB_ACT_NONE = 0,
+  CTB_ACT_RELU = 1,
+  CTB_ACT_GELU = 2,
+  CTB_ACT_GELU_TANH = 3,
+  CTB_ACT_SILU = 4
+} ctb_act;
+
+/* Z = A * B .+ bias, C = act.(Z) .+ R: ctb_gemm_f16 with an epilogue, for
+ * dtype F16 or BF16 and from one column of B (one token) up. Julia
+ * column-major: A is M x K (the weight), B is K x N (a column per token), C,
+ * R and Z are M x N; lda, ldb, ldr, ldz, ldc are column strides. bias: M
+ * elements of dtype bias_dtype (the matrices' or F32), or NULL; R (residual)
+ * may be NULL, and may be C itself; Z receives the value before the activation (what
+ * ctb_dense_bwd needs), or NULL. Sums, bias, activation and residual are
+ * Float32, rounded once to C (and once to Z). The result of a call does not
+ * depend on the schedule (no atomics). `workspace` (16-byte aligned) of at
+ * least ctb_dense_fwd_workspace_bytes() bytes, which is 0 when A and B start
+ * on 16-byte boundaries and lda and ldb are multiples of 8. */
+int64_t ctb_dense_fwd_workspace_bytes(const void* A, const void* B, int32_t M, int32_t N,
+                                      int32_t K, int64_t lda, int64_t ldb);
+int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const void* bias,
+                  int32_t bias_dtype, const void* R, void* Z, void* C, int32_t M, int32_t N,
+                  int32_t K, int64_t lda, int64_t ldb, int64_t ldr, int64_t ldz, int64_t ldc,
+                  int32_t act, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients of ctb_dense_fwd from dC (M x N): with dZ = dC .* act'(Z),
+ *   dA = dZ * B' (M x K),  dB = A' * dZ (K x N),  dbias = sum(dZ; dims=2) (M floats).
+ * Any of dA, dB, dbias may be NULL (not wanted). Z is the forward call's (not
+ * read where act is CTB_ACT_NONE). The gradient of the residual is dC. dZ is
+ * rounded to the matrices' type as an operand of the products; dbias is summed
+ * in Float32 from the unrounded values, in a fixed order. */
+int64_t ctb_dense_bwd_workspace_bytes(const void* dC, const void* A, const void* B, int32_t M,
+                                      int32_t N, int32_t K, int64_t lddc, int64_t lda,
+                                      int64_t ldb, int32_t act, int32_t need_dbias);
+int ctb_dense_bwd(int32_t dtype, const void* dC, const void* A, const void* B, const void* Z,
+                  void* dA, void* dB, float* dbias, int32_t M, int32_t N, int32_t K,
+                  int64_t lddc, int64_t lda, int64_t ldb, int64_t ldz, int64_t ldda,
+                  int64_t lddb, int32_t act, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+
 /* ---- mixture-of-experts layer: routing and combine -------------------------- */
 
 /* Scores of ctb_moe_route. */

@@ -18,6 +18,7 @@ layernorm with OpenMP; GEMM and attention are restated here in numpy float64
   reference (parity unpinned); restated from their standard definitions.
 """
 import ctypes
+import math
 import os
 import subprocess
 
@@ -250,6 +251,44 @@ def moe(A, B, sorted_ids, expert_ids, num_post_padded, topk, weights=None, block
             rows *= w[ids][:, None]
         C[ids] = rows
     return C
+
+
+def activation(z, act):
+    """Float64 (value, slope) of an activation of the dense layer."""
+    z = np.asarray(z, np.float64)
+    if act == "relu":
+        return np.maximum(z, 0), (z > 0).astype(np.float64)
+    if act == "silu":
+        s = 1 / (1 + np.exp(-z))
+        return z * s, s * (1 + z * (1 - s))
+    if act == "gelu":
+        erfc = np.vectorize(math.erfc, otypes=[np.float64])
+        cdf = 0.5 * erfc(-z / math.sqrt(2))
+        return z * cdf, cdf + z * np.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if act == "gelu_tanh":
+        c = math.sqrt(2 / math.pi)
+        th = np.tanh(c * (z + 0.044715 * z ** 3))
+        return (0.5 * z * (1 + th),
+                0.5 * (1 + th) + 0.5 * z * (1 - th * th) * c * (1 + 3 * 0.044715 * z * z))
+    return z, np.ones_like(z)
+
+
+def dense(A_t, B_t, bias=None, act="none", residual=None):
+    """Float64 (value, value before the activation) of the dense layer on Julia
+    column-major storage: A_t (K, M), B_t (N, K) -> (N, M)."""
+    z = np.asarray(B_t, np.float64) @ np.asarray(A_t, np.float64)
+    if bias is not None:
+        z = z + np.asarray(bias, np.float64)
+    y = activation(z, act)[0]
+    return (y if residual is None else y + np.asarray(residual, np.float64)), z
+
+
+def dense_bwd(dC_t, A_t, B_t, act="none", preact=None):
+    """Float64 gradients (dA_t, dB_t, dbias) and dZ of the dense layer."""
+    dz = np.asarray(dC_t, np.float64)
+    if act != "none":
+        dz = dz * activation(preact, act)[1]
+    return (np.asarray(B_t, np.float64).T @ dz, dz @ np.asarray(A_t, np.float64).T, dz.sum(0), dz)
 
 
 def moe_route(x, topk, score="softmax", bias=None, groups=1, topk_groups=None, group_top=2,
