@@ -132,6 +132,7 @@ int fmha_take_device_error(unsigned int* out);
 int moe_take_device_error(unsigned int* out);
 int layernorm_bwd_take_device_error(unsigned int* out);
 int selftest_take_device_error(unsigned int* out);
+int dense_take_device_error(unsigned int* out);
 }
 
 extern "C" int ctb_init(int device) {
@@ -198,7 +199,10 @@ extern "C" int ctb_check_device(void* stream) {
   unsigned int hs = 0;
   if (int e = selftest_take_device_error(&hs))
     return cuda_fail((cudaError_t)e, "reading the self-test error word");
-  const unsigned int h = hg | hf | hm | hl | hs;
+  unsigned int hd = 0;
+  if (int e = dense_take_device_error(&hd))
+    return cuda_fail((cudaError_t)e, "reading the dense layer's error word");
+  const unsigned int h = hg | hf | hm | hl | hs | hd;
   if (h) {
     return set_error(CTB_ERR_TIMEOUT, "a bounded device-side wait gave up (error word " +
                                           std::to_string(h) + ")");

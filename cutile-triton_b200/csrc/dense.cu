@@ -12,72 +12,83 @@
 
 namespace ctb {
 namespace dense {
+
+// dense_sm100.cu
+template <typename T>
+int product_sm100(const Product& p, cudaStream_t st);
+
 namespace {
 
-// ---- general product: any size, stride and alignment, on the CUDA cores ---------------
-// 256 threads; each computes a 4 x 4 block of a 64 x 64 tile of D.
-constexpr int SG = 64, SG_K = 16;
-
+// ---- a product over nothing: act(bias) + R ---------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256) product_simt_kernel(const Product p) {
-  __shared__ float Ps[SG_K][SG + 1];
-  __shared__ float Qs[SG_K][SG + 1];
-  const T* P = static_cast<const T*>(p.P);
-  const T* Q = static_cast<const T*>(p.Q);
-  const int64_t prs = p.p_mn ? 1 : p.ldp, pks = p.p_mn ? p.ldp : 1;
-  const int64_t qcs = p.q_mn ? 1 : p.ldq, qks = p.q_mn ? p.ldq : 1;
-  const int c0 = blockIdx.x * SG;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  for (int64_t r0 = (int64_t)blockIdx.y * SG; r0 < p.rows; r0 += (int64_t)gridDim.y * SG) {
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < p.depth; k0 += SG_K) {
-      for (int i = threadIdx.x; i < SG * SG_K; i += 256) {
-        const int a = p.p_mn ? i % SG : i / SG_K, ka = p.p_mn ? i / SG : i % SG_K;
-        Ps[ka][a] = r0 + a < p.rows && k0 + ka < p.depth
-                        ? to_f32(P[(r0 + a) * prs + (k0 + ka) * pks]) : 0.f;
-        const int b = p.q_mn ? i % SG : i / SG_K, kb = p.q_mn ? i / SG : i % SG_K;
-        Qs[kb][b] = c0 + b < p.cols && k0 + kb < p.depth
-                        ? to_f32(Q[(c0 + b) * qcs + (k0 + kb) * qks]) : 0.f;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < SG_K; ++k) {
-        float a[4], b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = Ps[k][ty + 16 * i];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = Qs[k][tx + 16 * j];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t r = r0 + ty + 16 * i;
-        const int c = c0 + tx + 16 * j;
-        if (r >= p.rows || c >= p.cols) continue;
-        float z = acc[i][j];
-        if (p.bias)
-          z += p.bias_f32 ? static_cast<const float*>(p.bias)[c]
-                          : to_f32(static_cast<const T*>(p.bias)[c]);
-        if (p.Z) from_f32(static_cast<T*>(p.Z) + r * p.ldz + c, z);
-        float v = activate_any(z, p.act);
-        if (p.R) v += to_f32(static_cast<const T*>(p.R)[r * p.ldr + c]);
-        from_f32(static_cast<T*>(p.D) + r * p.ldd + c, v);
-      }
+__global__ void __launch_bounds__(256) product_empty_kernel(const Product p) {
+  const int64_t total = (int64_t)p.rows * p.cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / p.cols;
+    const int c = (int)(i - r * p.cols);
+    float z = 0.f;
+    if (p.bias)
+      z = p.bias_f32 ? static_cast<const float*>(p.bias)[c] : to_f32(static_cast<const T*>(p.bias)[c]);
+    if (p.Z) from_f32(static_cast<T*>(p.Z) + r * p.ldz + c, z);
+    float v = activate_any(z, p.act);
+    if (p.R) v += to_f32(static_cast<const T*>(p.R)[r * p.ldr + c]);
+    from_f32(static_cast<T*>(p.D) + r * p.ldd + c, v);
   }
 }
 
+// ---- operands that TMA cannot address ----------------------------------------------------
+int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// A matrix of `lines` lines of `len` contiguous elements is addressable where
+// it starts on a 16-byte boundary and its lines do.
+bool tma_lines(const void* p, int64_t ld, int64_t lines) {
+  return aligned16(p) && (ld % 8 == 0 || lines <= 1);
+}
+int64_t packed_bytes(int64_t lines, int64_t len) { return round256(2 * lines * round8(len)); }
+
+// Copies lines of 16-bit elements to lines round8(len) apart. One thread per 16
+// bytes of the result.
+__global__ void __launch_bounds__(256)
+    pack_kernel(const uint16_t* __restrict__ src, uint4* __restrict__ dst, int64_t lines, int len,
+                int64_t ld) {
+  const int runs = (len + 7) / 8;
+  const int64_t total = lines * runs;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t l = i / runs;
+    const int c = (int)(i - l * runs) * 8;
+    const uint16_t* p = src + l * ld + c;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = c + 2 * j < len ? p[2 * j] : 0, hi = c + 2 * j + 1 < len ? p[2 * j + 1] : 0;
+      w[j] = lo | hi << 16;
+    }
+    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Replaces an operand that TMA cannot address by its copy at `ws`, which moves on.
+int pack_operand(const void** p, int64_t* ld, int64_t lines, int64_t len, uint8_t** ws, int sms,
+                 cudaStream_t st) {
+  if (lines == 0 || len == 0 || tma_lines(*p, *ld, lines)) return CTB_OK;
+  const int64_t grid = std::min<int64_t>((lines * ((len + 7) / 8) + 255) / 256, 16ll * sms);
+  pack_kernel<<<(unsigned)grid, 256, 0, st>>>(static_cast<const uint16_t*>(*p),
+                                              reinterpret_cast<uint4*>(*ws), lines, (int)len, *ld);
+  *p = *ws;
+  *ld = round8(len);
+  *ws += packed_bytes(lines, len);
+  return launch_status("pack_kernel");
+}
+
 template <typename T>
-int product(const Product& p, cudaStream_t st) {
-  const dim3 grid((p.cols + SG - 1) / SG, std::min((p.rows + SG - 1) / SG, 65535));
-  product_simt_kernel<T><<<grid, 256, 0, st>>>(p);
-  return launch_status("product_simt_kernel");
+int product(const Product& p, int sms, cudaStream_t st) {
+  if (p.depth > 0) return product_sm100<T>(p, st);
+  const int64_t grid = std::min<int64_t>(((int64_t)p.rows * p.cols + 255) / 256, 16ll * sms);
+  product_empty_kernel<T><<<(unsigned)grid, 256, 0, st>>>(p);
+  return launch_status("product_empty_kernel");
 }
 
 // ---- dZ = dC .* act'(Z) and its column sums ---------------------------------------------
@@ -130,52 +141,61 @@ __global__ void fold_kernel(const float* __restrict__ partial, float* __restrict
 constexpr int MAX_SPANS = 64;
 int spans_of(int N) { return std::max(1, std::min(MAX_SPANS, (N + 63) / 64)); }
 
-int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
-int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+// dZ goes to the workspace where it is not dC itself: with an activation, or
+// where TMA cannot address dC.
+bool dz_apart(const void* dC, int64_t lddc, int N, int act) {
+  return act != CTB_ACT_NONE || !tma_lines(dC, lddc, N);
+}
 
 template <typename T>
 int dense_bwd(const T* dC, const T* A, const T* B, const T* Z, T* dA, T* dB, float* dbias, int M,
               int N, int K, int64_t lddc, int64_t lda, int64_t ldb, int64_t ldz, int64_t ldda,
-              int64_t lddb, int act, uint8_t* ws, cudaStream_t st) {
-  const T* dZ = dC;
+              int64_t lddb, int act, uint8_t* ws, int sms, cudaStream_t st) {
+  const void* dZ = dC;
   int64_t lddz = lddc;
-  if (act != CTB_ACT_NONE || dbias) {
+  const bool products = (dA || dB) && K > 0;
+  const bool apart = products && dz_apart(dC, lddc, N, act);
+  if ((apart || dbias) && M > 0) {
     const int spans = spans_of(N);
     float* partial = reinterpret_cast<float*>(ws);
+    if (dbias) ws += round256(4ll * MAX_SPANS * M);
     T* dz = nullptr;
-    if (act != CTB_ACT_NONE) {
-      lddz = round8(M);
-      dz = reinterpret_cast<T*>(ws + (dbias ? round256(4ll * MAX_SPANS * M) : 0));
+    if (apart) {
+      dz = reinterpret_cast<T*>(ws);
+      ws += packed_bytes(N, M);
       dZ = dz;
+      lddz = round8(M);
     }
-    if (M > 0) {
-      const dim3 grid((M + SUM_COLS - 1) / SUM_COLS, spans);
-      slope_kernel<T><<<grid, SUM_THREADS, 0, st>>>(
-          dC, act != CTB_ACT_NONE ? Z : nullptr, dz, dbias ? (spans > 1 ? partial : dbias) : nullptr,
-          N, M, lddc, ldz, lddz, act, (N + spans - 1) / spans);
-      if (int rc = launch_status("slope_kernel")) return rc;
-      if (dbias && spans > 1) {
-        fold_kernel<<<(M + 255) / 256, 256, 0, st>>>(partial, dbias, M, spans);
-        if (int rc = launch_status("fold_kernel")) return rc;
-      }
+    const dim3 grid((M + SUM_COLS - 1) / SUM_COLS, spans);
+    slope_kernel<T><<<grid, SUM_THREADS, 0, st>>>(
+        dC, act != CTB_ACT_NONE ? Z : nullptr, dz, dbias ? (spans > 1 ? partial : dbias) : nullptr,
+        N, M, lddc, ldz, lddz, act, (N + spans - 1) / spans);
+    if (int rc = launch_status("slope_kernel")) return rc;
+    if (dbias && spans > 1) {
+      fold_kernel<<<(M + 255) / 256, 256, 0, st>>>(partial, dbias, M, spans);
+      if (int rc = launch_status("fold_kernel")) return rc;
     }
   }
   if (dB && N > 0 && K > 0) {
+    const void* q = A;
+    if (int rc = pack_operand(&q, &lda, K, M, &ws, sms, st)) return rc;
     Product p = {};
     p.P = dZ;
     p.ldp = lddz;
-    p.Q = A;
+    p.Q = q;
     p.ldq = lda;
     p.D = dB;
     p.ldd = lddb;
     p.rows = N;
     p.cols = K;
     p.depth = M;
-    if (int rc = product<T>(p, st)) return rc;
+    if (int rc = product<T>(p, sms, st)) return rc;
   }
   if (dA && M > 0 && K > 0) {
+    const void* q = B;
+    if (int rc = pack_operand(&q, &ldb, N, K, &ws, sms, st)) return rc;
     Product p = {};
-    p.P = B;
+    p.P = q;
     p.ldp = ldb;
     p.p_mn = true;
     p.Q = dZ;
@@ -186,7 +206,7 @@ int dense_bwd(const T* dC, const T* A, const T* B, const T* Z, T* dA, T* dB, flo
     p.rows = K;
     p.cols = M;
     p.depth = N;
-    if (int rc = product<T>(p, st)) return rc;
+    if (int rc = product<T>(p, sms, st)) return rc;
   }
   return CTB_OK;
 }
@@ -209,19 +229,22 @@ using namespace ctb;
 
 extern "C" int64_t ctb_dense_fwd_workspace_bytes(const void* A, const void* B, int32_t M, int32_t N,
                                                  int32_t K, int64_t lda, int64_t ldb) {
-  (void)A, (void)B, (void)M, (void)N, (void)K, (void)lda, (void)ldb;
-  return 0;
+  using namespace dense;
+  if (M < 0 || N < 0 || K < 0) return -1;
+  return (tma_lines(A, lda, K) ? 0 : packed_bytes(K, M)) +
+         (tma_lines(B, ldb, N) ? 0 : packed_bytes(N, K));
 }
 
 extern "C" int64_t ctb_dense_bwd_workspace_bytes(const void* dC, const void* A, const void* B,
                                                  int32_t M, int32_t N, int32_t K, int64_t lddc,
                                                  int64_t lda, int64_t ldb, int32_t act,
                                                  int32_t need_dbias) {
-  (void)dC, (void)A, (void)B, (void)K, (void)lddc, (void)lda, (void)ldb;
+  using namespace dense;
   if (M < 0 || N < 0 || K < 0) return -1;
-  int64_t b = need_dbias ? dense::round256(4ll * dense::MAX_SPANS * M) : 0;
-  if (act != CTB_ACT_NONE) b += dense::round256(2ll * N * dense::round8(M));
-  return b;
+  return (need_dbias ? round256(4ll * MAX_SPANS * M) : 0) +
+         (dz_apart(dC, lddc, N, act) ? packed_bytes(N, M) : 0) +
+         (tma_lines(A, lda, K) ? 0 : packed_bytes(K, M)) +
+         (tma_lines(B, ldb, N) ? 0 : packed_bytes(N, K));
 }
 
 extern "C" int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const void* bias,
@@ -262,7 +285,11 @@ extern "C" int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const 
   p.Z = Z;
   p.ldz = ldz;
   auto st = static_cast<cudaStream_t>(stream);
-  return dtype == CTB_F16 ? dense::product<__half>(p, st) : dense::product<__nv_bfloat16>(p, st);
+  auto* ws = static_cast<uint8_t*>(workspace);
+  if (int rc = dense::pack_operand(&p.P, &p.ldp, N, K, &ws, pr.sm_count, st)) return rc;
+  if (int rc = dense::pack_operand(&p.Q, &p.ldq, K, M, &ws, pr.sm_count, st)) return rc;
+  return dtype == CTB_F16 ? dense::product<__half>(p, pr.sm_count, st)
+                          : dense::product<__nv_bfloat16>(p, pr.sm_count, st);
 }
 
 extern "C" int ctb_dense_bwd(int32_t dtype, const void* dC, const void* A, const void* B,
@@ -291,9 +318,9 @@ extern "C" int ctb_dense_bwd(int32_t dtype, const void* dC, const void* A, const
   if (dtype == CTB_F16)
     return dense::dense_bwd<__half>((const __half*)dC, (const __half*)A, (const __half*)B,
                                     (const __half*)Z, (__half*)dA, (__half*)dB, dbias, M, N, K,
-                                    lddc, lda, ldb, ldz, ldda, lddb, act, ws, st);
+                                    lddc, lda, ldb, ldz, ldda, lddb, act, ws, pr.sm_count, st);
   using bf = __nv_bfloat16;
   return dense::dense_bwd<bf>((const bf*)dC, (const bf*)A, (const bf*)B, (const bf*)Z, (bf*)dA,
                               (bf*)dB, dbias, M, N, K, lddc, lda, ldb, ldz, ldda, lddb, act, ws,
-                              st);
+                              pr.sm_count, st);
 }
