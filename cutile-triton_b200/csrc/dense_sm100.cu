@@ -10,10 +10,18 @@
 // partials over distributed shared memory and add them in rank order, each
 // finishing (bias, activation, residual, rounding) its share of the tile. No
 // workspace, no atomics, the same result every time.
+//
+// product_pair_kernel: 256 x 256 tiles over two SMs (tcgen05 cta_group::2),
+// persistent, for products with tiles enough to fill the GPU. Here the rows of D
+// are the tensor cores' M side: a thread of the epilogue then holds neighbouring
+// columns of one row, which move through swizzled shared memory as 16-byte
+// pieces and in and out of it by TMA, and the bias is the same for all lanes.
 #include "dense.cuh"
 #include "sm100_ptx.cuh"
 
 #include <algorithm>
+#include <cstdlib>
+#include <cstring>
 #include <mutex>
 
 namespace ctb {
@@ -298,9 +306,383 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
   if (S > 1) cluster_sync_all();  // no CTA leaves while a peer may read its partials
 }
 
+// ---- pair kernel -----------------------------------------------------------------------
+// Warps: 0 TMA producer, 1 TMEM owner and MMA issuer (even CTA), 2..9 epilogue:
+// two per quarter of the TMEM lanes, 128 columns each, so that an activation of
+// 40 instructions an element still hides under a main loop of 1024 k.
+// Each CTA loads its own 128 rows of P and 128 columns of Q (32 KB a k-block, 5
+// stages); two 256-column accumulators let a tile's epilogue run under the next
+// tile's main loop. Barriers as in gemm_sm100.cu: full[] and tmem_empty[] in the
+// even CTA, empty[] and tmem_full[] in both.
+constexpr int PR_THREADS = 320;
+constexpr int PR_STAGES = 5;
+constexpr int PR_OP_BYTES = 128 * BK * 2;
+constexpr int PR_STAGE_BYTES = 2 * PR_OP_BYTES;
+constexpr int PR_WARPS = 8;                   // epilogue warps
+constexpr int PR_BOX = 32 * 32 * 2;           // 32 rows x 32 columns, 64-byte swizzle
+constexpr int PR_BOXES = 4;                   // per warp: 2 for stores, 2 for the residual
+constexpr int PR_SMEM = PR_STAGES * PR_STAGE_BYTES + PR_WARPS * PR_BOXES * PR_BOX +
+                        PR_WARPS * 32 * 4 + 1024 + 512;
+constexpr int PR_GROUP = 8;                   // row tiles per group of the tile order
+
+struct PairArgs {
+  Epilogue e;
+  int num_kb, tiles_r, tiles_c;
+  int64_t num_tiles;
+  bool d_tma, z_tma, r_tma;
+};
+
+__device__ __forceinline__ void pair_tile(const PairArgs& p, int64_t t, int& tr, int& tc) {
+  const int64_t span = (int64_t)PR_GROUP * p.tiles_c;
+  const int64_t g = t / span;
+  const int first = (int)g * PR_GROUP;
+  const int size = min(p.tiles_r - first, PR_GROUP);
+  const int rest = (int)(t - g * span);
+  tr = first + rest % size;
+  tc = rest / size;
+}
+
+// Byte offset of 16-byte piece `piece` (0..3) of row `row` in a 64-byte-swizzled box.
+__device__ __forceinline__ int box_at(int row, int piece) {
+  return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4);
+}
+
+template <typename T, int ACT>
+__device__ __forceinline__ void activate32(uint32_t (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    v[j] = __float_as_uint(activate<ACT>(__uint_as_float(v[j])));
+}
+
+template <typename T, bool P_MN, bool Q_MN>
+__global__ void __launch_bounds__(PR_THREADS, 1)
+    product_pair_kernel(const __grid_constant__ CUtensorMap tmP,
+                        const __grid_constant__ CUtensorMap tmQ,
+                        const __grid_constant__ CUtensorMap tmD,
+                        const __grid_constant__ CUtensorMap tmZ,
+                        const __grid_constant__ CUtensorMap tmR, const PairArgs a) {
+  using namespace sm100;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint8_t* boxes = smem + PR_STAGES * PR_STAGE_BYTES;
+  float* bias_all = reinterpret_cast<float*>(boxes + PR_WARPS * PR_BOXES * PR_BOX);
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_all + PR_WARPS * 32);
+  uint64_t* empty = full + PR_STAGES;
+  uint64_t* tmem_full = empty + PR_STAGES;  // [2]
+  uint64_t* tmem_empty = tmem_full + 2;     // [2]
+  uint64_t* r_full = tmem_empty + 2;        // [PR_WARPS][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_full + 2 * PR_WARPS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int64_t pair = blockIdx.x / 2, num_pairs = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < PR_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tmem_full[i], 1);
+      mbar_init(&tmem_empty[i], 2 * PR_WARPS * 32);
+    }
+    for (int i = 0; i < 2 * PR_WARPS; ++i) mbar_init(&r_full[i], 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmP);
+    tma_prefetch_desc(&tmQ);
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before();
+  cluster_sync_all();  // barriers initialised in both CTAs before any cross-CTA use
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t full_leader = mapa_shared(smem_u32(&full[0]), 0);
+
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int64_t issued = 0;
+      bool ok = true;
+      for (int64_t t = pair; ok && t < a.num_tiles && !*abort_flag; t += num_pairs) {
+        int tr, tc;
+        pair_tile(a, t, tr, tc);
+        const int r0 = tr * 256 + (int)rank * 128, c0 = tc * 256 + (int)rank * 128;
+        for (int kb = 0; kb < a.num_kb; ++kb) {
+          if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, ERR_BIT))) break;
+          uint8_t* sp = smem + stage * PR_STAGE_BYTES;
+          uint8_t* sq = sp + PR_OP_BYTES;
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * PR_STAGE_BYTES);
+          const uint32_t bar = full_leader + stage * 8;
+          if (P_MN) {
+            tma_load_2d_pair(sp, &tmP, bar, r0, kb * BK);
+            tma_load_2d_pair(sp + PR_OP_BYTES / 2, &tmP, bar, r0 + 64, kb * BK);
+          } else {
+            tma_load_2d_pair(sp, &tmP, bar, kb * BK, r0);
+          }
+          if (Q_MN) {
+            tma_load_2d_pair(sq, &tmQ, bar, c0, kb * BK);
+            tma_load_2d_pair(sq + PR_OP_BYTES / 2, &tmQ, bar, c0 + 64, kb * BK);
+          } else {
+            tma_load_2d_pair(sq, &tmQ, bar, kb * BK, c0);
+          }
+          ++issued;
+          if (++stage == PR_STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // The even CTA's barriers count both CTAs' loads; the other stays until
+      // the cluster barrier below.
+      if (*abort_flag && leader) drain_loads(full, issued, PR_STAGES);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (even CTA only) ----------------
+    if (leader) {
+      constexpr uint32_t idesc = idesc_f16_f32(256, 256, P_MN, Q_MN) | Format<T>::idesc;
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;
+      bool ok = true;
+      for (int64_t t = pair; ok && t < a.num_tiles; t += num_pairs, ++it) {
+        const int buf = it & 1;
+        const uint32_t acc_phase = (it >> 1) & 1;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&tmem_empty[buf], acc_phase ^ 1,
+                                                             abort_flag, ERR_BIT))))
+          break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * 256;
+        for (int kb = 0; kb < a.num_kb; ++kb) {
+          if (!(ok = __all_sync(0xffffffffu,
+                                mbar_wait_bounded(&full[stage], phase, abort_flag, ERR_BIT))))
+            break;
+          tc_fence_after();
+          const uint32_t sp = smem_u32(smem + stage * PR_STAGE_BYTES);
+          const uint64_t pd = smem_desc_sw128(sp, P_MN ? 8192 : 16, 1024);
+          const uint64_t qd = smem_desc_sw128(sp + PR_OP_BYTES, Q_MN ? 8192 : 16, 1024);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            mma_f16_ss_pair_elect(d_tmem, pd + (uint64_t)((P_MN ? 2048 : 32) * k >> 4),
+                                  qd + (uint64_t)((Q_MN ? 2048 : 32) * k >> 4), idesc,
+                                  (kb | k) != 0);
+          mma_commit_pair_both_elect(&empty[stage]);
+          if (++stage == PR_STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        mma_commit_pair_both_elect(&tmem_full[buf]);
+      }
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    const int q = warp & 3, half = (warp - 2) >> 2, w = warp - 2;
+    const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+    uint8_t* box = boxes + w * PR_BOXES * PR_BOX;
+    float* bias_s = bias_all + w * 32;
+    uint64_t* rbar = r_full + 2 * w;
+    const uint32_t tmem_empty_leader = mapa_shared(smem_u32(&tmem_empty[0]), 0);
+    const Epilogue& e = a.e;
+    const bool all_tma = a.d_tma && (!e.Z || a.z_tma);
+    int sbuf = 0;
+    uint32_t r_issued = 0, r_used = 0;  // residual boxes asked for and read
+    int it = 0;
+
+    // Rows r0.. and columns c.. of this warp's chunk `i` (32 columns) of tile t.
+    auto fetch_residual = [&](int r0, int c) {
+      if (lane == 0) {
+        uint64_t* bar = &rbar[r_issued & 1];
+        mbar_arrive_expect_tx(bar, PR_BOX);
+        tma_load_2d(box + (2 + (r_issued & 1)) * PR_BOX, &tmR, bar, c, r0);
+      }
+      ++r_issued;
+    };
+    auto put = [&](const uint32_t (&v)[32], const CUtensorMap* map, void* base, int64_t ld,
+                   bool tma, int r0, int c) {
+      uint8_t* b = box + sbuf * PR_BOX;
+      // This box's previous store has read it: the last store but one where all
+      // go by TMA, else possibly the last.
+      if (lane == 0) {
+        if (all_tma) bulk_wait_read<1>();
+        else bulk_wait_read<0>();
+      }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[8 * j + i]);
+        *reinterpret_cast<uint4*>(b + box_at(lane, j)) = pack8<T>(f);
+      }
+      if (tma) {
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(map, b, c, r0);
+          bulk_commit();
+        }
+      } else {
+        __syncwarp();
+        T* out = static_cast<T*>(base) + (int64_t)r0 * ld + c + lane;
+        if (c + lane < e.cols)
+          for (int r = 0; r < 32 && r0 + r < e.rows; ++r)
+            out[r * ld] = *reinterpret_cast<const T*>(b + box_at(r, lane >> 3) + (lane & 7) * 2);
+        __syncwarp();
+      }
+      sbuf ^= 1;
+    };
+
+    for (int64_t t = pair; t < a.num_tiles && !*abort_flag; t += num_pairs, ++it) {
+      const int buf = it & 1;
+      const uint32_t acc_phase = (it >> 1) & 1;
+      int tr, tc;
+      pair_tile(a, t, tr, tc);
+      const int r0 = tr * 256 + (int)rank * 128 + q * 32;
+      const int c0 = tc * 256 + half * 128;
+      // Chunks of this tile that hold any of D (a prefix of the four).
+      const int chunks = r0 < e.rows && c0 < e.cols ? min(4, (e.cols - c0 + 31) / 32) : 0;
+      const bool by_tma = e.R && a.r_tma;
+      if (by_tma)
+        for (int i = 0; i < min(2, chunks); ++i) fetch_residual(r0, c0 + 32 * i);
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait_bounded(&tmem_full[buf], acc_phase, abort_flag, ERR_BIT)))
+        break;
+      tc_fence_after();
+      const uint32_t tcol = tmem_base + buf * 256 + half * 128 + lane_base;
+      bool ok = true;
+      auto finish = [&](uint32_t (&v)[32], int i) {
+        if (i >= chunks) return;
+        const int c = c0 + 32 * i;
+        if (e.bias) {
+          bias_s[lane] = c + lane >= e.cols ? 0.f
+                         : e.bias_f32 ? static_cast<const float*>(e.bias)[c + lane]
+                                      : to_f32(static_cast<const T*>(e.bias)[c + lane]);
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 b = reinterpret_cast<const float4*>(bias_s)[j];
+            v[4 * j + 0] = __float_as_uint(__uint_as_float(v[4 * j + 0]) + b.x);
+            v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + b.y);
+            v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + b.z);
+            v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + b.w);
+          }
+          __syncwarp();
+        }
+        if (e.Z) put(v, &tmZ, e.Z, e.ldz, a.z_tma, r0, c);
+        switch (e.act) {
+          case CTB_ACT_RELU: activate32<T, CTB_ACT_RELU>(v); break;
+          case CTB_ACT_GELU: activate32<T, CTB_ACT_GELU>(v); break;
+          case CTB_ACT_GELU_TANH: activate32<T, CTB_ACT_GELU_TANH>(v); break;
+          case CTB_ACT_SILU: activate32<T, CTB_ACT_SILU>(v); break;
+          default: break;
+        }
+        if (e.R) {
+          uint8_t* b = box + (2 + (by_tma ? r_used & 1 : 0)) * PR_BOX;
+          if (by_tma) {
+            ok &= (bool)__all_sync(0xffffffffu,
+                                   mbar_wait_bounded(&rbar[r_used & 1], (r_used >> 1) & 1,
+                                                     abort_flag, ERR_BIT));
+            ++r_used;
+          } else {
+            const T* in = static_cast<const T*>(e.R) + (int64_t)r0 * e.ldr + c + lane;
+            if (c + lane < e.cols)
+              for (int r = 0; r < 32 && r0 + r < e.rows; ++r)
+                *reinterpret_cast<T*>(b + box_at(r, lane >> 3) + (lane & 7) * 2) = in[r * e.ldr];
+            __syncwarp();
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float f[8];
+            unpack8<T>(*reinterpret_cast<const uint4*>(b + box_at(lane, j)), f);
+#pragma unroll
+            for (int i2 = 0; i2 < 8; ++i2)
+              v[8 * j + i2] = __float_as_uint(__uint_as_float(v[8 * j + i2]) + f[i2]);
+          }
+          __syncwarp();
+          if (by_tma && i + 2 < chunks) fetch_residual(r0, c + 64);
+        }
+        put(v, &tmD, e.D, e.ldd, a.d_tma, r0, c);
+      };
+      uint32_t ra[32], rb[32];
+      tmem_ld_32x32b_x32(tcol, ra);
+#pragma unroll 1
+      for (int i = 0; i < 4; i += 2) {
+        tmem_ld_wait_regs(ra);
+        tmem_ld_32x32b_x32(tcol + 32 * (i + 1), rb);
+        finish(ra, i);
+        tmem_ld_wait_regs(rb);
+        if (i + 2 < 4) {
+          tmem_ld_32x32b_x32(tcol + 32 * (i + 2), ra);
+        } else {
+          // The accumulator is in registers: the next tile but one may have it.
+          tc_fence_before();
+          if (leader) mbar_arrive(&tmem_empty[buf]);
+          else mbar_arrive_cluster(tmem_empty_leader + buf * 8);
+        }
+        finish(rb, i + 1);
+      }
+      if (!ok) break;
+    }
+    if (lane == 0) {
+      for (; r_used < r_issued; ++r_used) {  // only after a wait that gave up
+        const uint64_t t0 = global_ns();
+        while (!mbar_try_wait_sleep(&rbar[r_used & 1], (r_used >> 1) & 1, 20000u) &&
+               global_ns() - t0 < 1000000000ull) {
+        }
+      }
+      bulk_wait<0>();  // staged boxes must outlive their stores
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  cluster_sync_all();  // no CTA leaves while its peer may still touch its shared memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------
 static unsigned long long g_dense_ctx[64];  // context ID the set-up was done in
+static int g_dense_pairs[64];               // CTA pairs that are resident at once
 static std::mutex g_dense_mu;
+
+template <typename T, bool P_MN, bool Q_MN>
+int pair_attr() {
+  CTB_CUDA_CHECK(cudaFuncSetAttribute(product_pair_kernel<T, P_MN, Q_MN>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, PR_SMEM));
+  return CTB_OK;
+}
+template <typename T>
+int pair_attrs() {
+  int rc = pair_attr<T, false, true>();
+  if (!rc) rc = pair_attr<T, false, false>();
+  if (!rc) rc = pair_attr<T, true, true>();
+  return rc;
+}
+static void cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, dim3 grid,
+                           int threads, int smem, int cluster, cudaStream_t st) {
+  *cfg = {};
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = cluster;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+  cfg->gridDim = grid;
+  cfg->blockDim = dim3(threads, 1, 1);
+  cfg->dynamicSmemBytes = smem;
+  cfg->stream = st;
+  cfg->attrs = attr;
+  cfg->numAttrs = 1;
+}
 
 template <typename T, bool Q_MN, bool P_MN, int BN>
 int split_attr() {
@@ -333,7 +715,17 @@ int device_setup() {
   if (dev < 64 && g_dense_ctx[dev] == ctx) return CTB_OK;
   if (int rc = split_attrs<__half>()) return rc;
   if (int rc = split_attrs<__nv_bfloat16>()) return rc;
-  if (dev < 64) g_dense_ctx[dev] = ctx;
+  if (int rc = pair_attrs<__half>()) return rc;
+  if (int rc = pair_attrs<__nv_bfloat16>()) return rc;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  cluster_config(&cfg, &attr, dim3(2), PR_THREADS, PR_SMEM, 2, nullptr);
+  int pairs = 0;
+  CTB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&pairs, product_pair_kernel<__half, false, true>, &cfg));
+  if (dev < 64) {
+    g_dense_pairs[dev] = pairs;
+    g_dense_ctx[dev] = ctx;
+  }
   return CTB_OK;
 }
 
@@ -346,6 +738,15 @@ int operand_map(CUtensorMap* m, const void* base, int64_t ld, bool mn, int exten
   const uint64_t strides[1] = {(uint64_t)ld * 2};
   const uint32_t box[2] = {64, (uint32_t)(mn ? 64 : box_rows)};
   return encode_tmap(m, Format<T>::map, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// CTB_DENSE_PAIR_TILES=n: the pair kernel from n tiles on (a measuring aid).
+static int pair_min_tiles() {
+  static const int n = [] {
+    const char* v = getenv("CTB_DENSE_PAIR_TILES");
+    return v ? atoi(v) : -1;
+  }();
+  return n;
 }
 
 static bool rows16(const void* p, int64_t ld, int rows) {
@@ -365,20 +766,52 @@ int split_launch(const Product& p, const Epilogue& e, int sms, cudaStream_t st) 
   // As many CTAs per tile as fill two per SM once, with 2 k-blocks each at least.
   int S = (int)std::max<int64_t>(1, std::min<int64_t>(8, 2ll * sms / (tiles_c * tiles_r)));
   S = std::max(1, std::min(S, a.num_kb / 2));
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = S;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(tiles_c * S), (unsigned)tiles_r, 1);
-  cfg.blockDim = dim3(SP_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = sp_smem(BN);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  cluster_config(&cfg, &attr, dim3((unsigned)(tiles_c * S), (unsigned)tiles_r, 1), SP_THREADS,
+                 sp_smem(BN), S, st);
   CTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, product_split_kernel<T, Q_MN, P_MN, BN>, tmQ, tmP, a));
   return launch_status("product_split_kernel");
+}
+
+// A 16-bit matrix as boxes of 32 rows x 32 columns for the epilogue; a matrix
+// that is not there, or that TMA cannot address, gets an empty map.
+template <typename T>
+int box_map(CUtensorMap* m, const void* base, int64_t ld, int rows, int cols, bool usable) {
+  if (!usable) {
+    std::memset(m, 0, sizeof(*m));
+    return CTB_OK;
+  }
+  const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows};
+  const uint64_t strides[1] = {(uint64_t)(rows > 1 ? ld : (cols + 7) / 8 * 8) * 2};
+  const uint32_t box[2] = {32, 32};
+  return encode_tmap(m, Format<T>::map, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+template <typename T, bool P_MN, bool Q_MN>
+int pair_launch(const Product& p, const Epilogue& e, int pairs, cudaStream_t st) {
+  CUtensorMap tmP, tmQ, tmD, tmZ, tmR;
+  PairArgs a;
+  a.e = e;
+  a.d_tma = rows16(p.D, p.ldd, p.rows);
+  a.z_tma = p.Z && rows16(p.Z, p.ldz, p.rows);
+  a.r_tma = p.R && rows16(p.R, p.ldr, p.rows);
+  if (int rc = operand_map<T>(&tmP, p.P, p.ldp, P_MN, p.rows, p.depth, 128)) return rc;
+  if (int rc = operand_map<T>(&tmQ, p.Q, p.ldq, Q_MN, p.cols, p.depth, 128)) return rc;
+  if (int rc = box_map<T>(&tmD, p.D, p.ldd, p.rows, p.cols, a.d_tma)) return rc;
+  if (int rc = box_map<T>(&tmZ, p.Z, p.ldz, p.rows, p.cols, a.z_tma)) return rc;
+  if (int rc = box_map<T>(&tmR, p.R, p.ldr, p.rows, p.cols, a.r_tma)) return rc;
+  a.num_kb = (p.depth + BK - 1) / BK;
+  a.tiles_r = (p.rows + 255) / 256;
+  a.tiles_c = (p.cols + 255) / 256;
+  a.num_tiles = (int64_t)a.tiles_r * a.tiles_c;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  cluster_config(&cfg, &attr, dim3((unsigned)(2 * std::min<int64_t>(a.num_tiles, pairs))),
+                 PR_THREADS, PR_SMEM, 2, st);
+  CTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, product_pair_kernel<T, P_MN, Q_MN>, tmP, tmQ, tmD, tmZ,
+                                    tmR, a));
+  return launch_status("product_pair_kernel");
 }
 
 // The product on the tensor cores. Operands start on 16-byte boundaries, their
@@ -407,6 +840,16 @@ int product_sm100(const Product& p0, cudaStream_t st) {
   e.vec = rows16(p.D, p.ldd, p.rows) && (!p.Z || rows16(p.Z, p.ldz, p.rows)) &&
           (!p.R || rows16(p.R, p.ldr, p.rows));
   const int sms = pr.sm_count;
+  int dev = 0;
+  CTB_CUDA_CHECK(cudaGetDevice(&dev));
+  const int pairs = dev < 64 ? g_dense_pairs[dev] : 0;
+  const int64_t pair_tiles = (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
+  const int min_tiles = pair_min_tiles() >= 0 ? pair_min_tiles() : pairs / 2;
+  if (pairs > 0 && pair_tiles >= std::max(1, min_tiles)) {
+    if (p.p_mn) return pair_launch<T, true, true>(p, e, pairs, st);
+    if (p.q_mn) return pair_launch<T, false, true>(p, e, pairs, st);
+    return pair_launch<T, false, false>(p, e, pairs, st);
+  }
   if (p.p_mn) {
     if (p.rows <= 64) return split_launch<T, true, true, 64>(p, e, sms, st);
     return split_launch<T, true, true, 128>(p, e, sms, st);
