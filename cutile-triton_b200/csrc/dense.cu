@@ -92,54 +92,131 @@ int product(const Product& p, int sms, cudaStream_t st) {
 }
 
 // ---- dZ = dC .* act'(Z) and its column sums ---------------------------------------------
-// A CTA takes SUM_COLS columns and a span of rows; spans are summed afterwards
-// in order, so the result does not depend on the schedule.
-constexpr int SUM_COLS = 64, SUM_THREADS = 256, SUM_LANES = SUM_THREADS / SUM_COLS;
+// One pass over dC and Z, bound by HBM. A warp takes 32 runs of W neighbouring
+// columns (16 bytes a lane where the rows allow it), a CTA eight rows at a time
+// of one strip, four of them in flight per warp; a lane keeps its columns' sums.
+// The strip's rows are split into spans so that every SM has six CTAs' worth;
+// spans are summed afterwards in order, so the result does not depend on the
+// schedule.
+constexpr int SLOPE_THREADS = 256, SLOPE_WARPS = SLOPE_THREADS / 32, SLOPE_FLIGHT = 4;
+constexpr int SLOPE_CTAS = 6 * 148;
 
-template <typename T>
-__global__ void __launch_bounds__(SUM_THREADS)
+template <typename T, int W> struct Columns;
+template <typename T> struct Columns<T, 8> {
+  uint4 raw;
+  __device__ void load(const T* p) { raw = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ void get(float (&f)[8]) const { unpack8<T>(raw, f); }
+  static __device__ void put(T* p, const float (&f)[8]) {
+    *reinterpret_cast<uint4*>(p) = pack8<T>(f);
+  }
+};
+template <typename T> struct Columns<T, 1> {
+  T v;
+  __device__ void load(const T* p) { v = *p; }
+  __device__ void get(float (&f)[1]) const { f[0] = to_f32(v); }
+  static __device__ void put(T* p, const float (&f)[1]) { from_f32(p, f[0]); }
+};
+
+template <typename T, int W, int ACT>
+__global__ void __launch_bounds__(SLOPE_THREADS)
     slope_kernel(const T* __restrict__ dC, const T* __restrict__ Z, T* __restrict__ dZ,
                  float* __restrict__ partial, int N, int M, int64_t lddc, int64_t ldz,
-                 int64_t lddz, int act, int span) {
-  __shared__ float red[SUM_LANES][SUM_COLS];
-  const int cl = threadIdx.x % SUM_COLS, rl = threadIdx.x / SUM_COLS;
-  const int c = blockIdx.x * SUM_COLS + cl;
+                 int64_t lddz, int span) {
+  __shared__ float red[SLOPE_WARPS][32 * W];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int c = (int)(blockIdx.x * 32 + lane) * W;
   const int64_t n0 = (int64_t)blockIdx.y * span, n1 = min((int64_t)N, n0 + span);
-  float sum = 0.f;
-  if (c < M)
-    for (int64_t n = n0 + rl; n < n1; n += SUM_LANES) {
-      float d = to_f32(dC[n * lddc + c]);
-      if (Z) {
-        const float z = to_f32(Z[n * ldz + c]);
-        switch (act) {
-          case CTB_ACT_RELU: d *= activate_slope<CTB_ACT_RELU>(z); break;
-          case CTB_ACT_GELU: d *= activate_slope<CTB_ACT_GELU>(z); break;
-          case CTB_ACT_GELU_TANH: d *= activate_slope<CTB_ACT_GELU_TANH>(z); break;
-          default: d *= activate_slope<CTB_ACT_SILU>(z); break;
+  float sum[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) sum[i] = 0.f;
+  if (c < M) {
+    for (int64_t n = n0 + warp; n < n1; n += SLOPE_WARPS * SLOPE_FLIGHT) {
+      Columns<T, W> d[SLOPE_FLIGHT], z[SLOPE_FLIGHT];
+#pragma unroll
+      for (int j = 0; j < SLOPE_FLIGHT; ++j) {
+        const int64_t r = n + j * SLOPE_WARPS;
+        if (r < n1) {
+          d[j].load(dC + r * lddc + c);
+          if (ACT != CTB_ACT_NONE) z[j].load(Z + r * ldz + c);
         }
       }
-      if (dZ) from_f32(dZ + n * lddz + c, d);
-      sum += d;
+#pragma unroll
+      for (int j = 0; j < SLOPE_FLIGHT; ++j) {
+        const int64_t r = n + j * SLOPE_WARPS;
+        if (r < n1) {
+          float f[W], s[W];
+          d[j].get(f);
+          if (ACT != CTB_ACT_NONE) {
+            z[j].get(s);
+            if (W == 1) {
+              float unused = 0.f;
+              slope2<ACT>(s[0], unused);
+            } else {
+#pragma unroll
+              for (int i = 0; i + 1 < W; i += 2) slope2<ACT>(s[i], s[i + 1]);
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) f[i] *= s[i];
+          }
+#pragma unroll
+          for (int i = 0; i < W; ++i) sum[i] += f[i];
+          if (dZ) Columns<T, W>::put(dZ + r * lddz + c, f);
+        }
+      }
     }
-  red[rl][cl] = sum;
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int i = 0; i < W; ++i) red[warp][lane * W + i] = sum[i];
   __syncthreads();
-  if (partial && rl == 0 && c < M) {
-    for (int i = 1; i < SUM_LANES; ++i) sum += red[i][cl];
-    partial[(int64_t)blockIdx.y * M + c] = sum;
+  for (int i = threadIdx.x; i < 32 * W; i += SLOPE_THREADS) {
+    const int col = (int)blockIdx.x * 32 * W + i;
+    float t = red[0][i];
+#pragma unroll
+    for (int w = 1; w < SLOPE_WARPS; ++w) t += red[w][i];
+    if (col < M) partial[(int64_t)blockIdx.y * M + col] = t;
   }
 }
 
-__global__ void fold_kernel(const float* __restrict__ partial, float* __restrict__ out, int M,
-                            int spans) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= M) return;
+// Sums the spans: 32 columns a CTA, eight threads a column, joined in order.
+__global__ void __launch_bounds__(256)
+    fold_kernel(const float* __restrict__ partial, float* __restrict__ out, int M, int spans) {
+  __shared__ float red[8][32];
+  const int cl = threadIdx.x % 32, g = threadIdx.x / 32, c = blockIdx.x * 32 + cl;
   float s = 0.f;
-  for (int i = 0; i < spans; ++i) s += partial[(int64_t)i * M + c];
-  out[c] = s;
+  if (c < M)
+#pragma unroll 8
+    for (int i = g; i < spans; i += 8) s += partial[(int64_t)i * M + c];
+  red[g][cl] = s;
+  __syncthreads();
+  if (g == 0 && c < M) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[i][cl];
+    out[c] = s;
+  }
 }
 
-constexpr int MAX_SPANS = 64;
-int spans_of(int N) { return std::max(1, std::min(MAX_SPANS, (N + 63) / 64)); }
+// Spans of the rows: 32 rows at least, at most what gives SLOPE_CTAS CTAs.
+int spans_of(int N, int M) {
+  const int strips = std::max(1, (M + 255) / 256);
+  return std::max(1, std::min((N + 31) / 32, SLOPE_CTAS / strips));
+}
+
+template <typename T, int W>
+int slope_launch(const T* dC, const T* Z, T* dZ, float* sums, int N, int M, int64_t lddc,
+                 int64_t ldz, int64_t lddz, int act, int spans, cudaStream_t st) {
+  const dim3 grid((M + 32 * W - 1) / (32 * W), spans);
+  auto k = slope_kernel<T, W, CTB_ACT_NONE>;
+  switch (act) {
+    case CTB_ACT_RELU: k = slope_kernel<T, W, CTB_ACT_RELU>; break;
+    case CTB_ACT_GELU: k = slope_kernel<T, W, CTB_ACT_GELU>; break;
+    case CTB_ACT_GELU_TANH: k = slope_kernel<T, W, CTB_ACT_GELU_TANH>; break;
+    case CTB_ACT_SILU: k = slope_kernel<T, W, CTB_ACT_SILU>; break;
+    default: break;
+  }
+  k<<<grid, SLOPE_THREADS, 0, st>>>(dC, Z, dZ, sums, N, M, lddc, ldz, lddz, (N + spans - 1) / spans);
+  return launch_status("slope_kernel");
+}
 
 // dZ goes to the workspace where it is not dC itself: with an activation, or
 // where TMA cannot address dC.
@@ -156,9 +233,10 @@ int dense_bwd(const T* dC, const T* A, const T* B, const T* Z, T* dA, T* dB, flo
   const bool products = (dA || dB) && K > 0;
   const bool apart = products && dz_apart(dC, lddc, N, act);
   if ((apart || dbias) && M > 0) {
-    const int spans = spans_of(N);
-    float* partial = reinterpret_cast<float*>(ws);
-    if (dbias) ws += round256(4ll * MAX_SPANS * M);
+    const int spans = spans_of(N, M);
+    float* sums = dbias;
+    if (dbias && spans > 1) sums = reinterpret_cast<float*>(ws);
+    if (dbias) ws += round256(4ll * spans * M);
     T* dz = nullptr;
     if (apart) {
       dz = reinterpret_cast<T*>(ws);
@@ -166,14 +244,14 @@ int dense_bwd(const T* dC, const T* A, const T* B, const T* Z, T* dA, T* dB, flo
       dZ = dz;
       lddz = round8(M);
     }
-    const dim3 grid((M + SUM_COLS - 1) / SUM_COLS, spans);
-    slope_kernel<T><<<grid, SUM_THREADS, 0, st>>>(
-        dC, act != CTB_ACT_NONE ? Z : nullptr, dz, dbias ? (spans > 1 ? partial : dbias) : nullptr,
-        N, M, lddc, ldz, lddz, act, (N + spans - 1) / spans);
-    if (int rc = launch_status("slope_kernel")) return rc;
+    const bool runs = M % 8 == 0 && tma_lines(dC, lddc, N) &&
+                      (act == CTB_ACT_NONE || tma_lines(Z, ldz, N));
+    int rc = runs ? slope_launch<T, 8>(dC, Z, dz, sums, N, M, lddc, ldz, lddz, act, spans, st)
+                  : slope_launch<T, 1>(dC, Z, dz, sums, N, M, lddc, ldz, lddz, act, spans, st);
+    if (rc) return rc;
     if (dbias && spans > 1) {
-      fold_kernel<<<(M + 255) / 256, 256, 0, st>>>(partial, dbias, M, spans);
-      if (int rc = launch_status("fold_kernel")) return rc;
+      fold_kernel<<<(M + 31) / 32, 256, 0, st>>>(sums, dbias, M, spans);
+      if ((rc = launch_status("fold_kernel"))) return rc;
     }
   }
   if (dB && N > 0 && K > 0) {
@@ -241,7 +319,7 @@ extern "C" int64_t ctb_dense_bwd_workspace_bytes(const void* dC, const void* A, 
                                                  int32_t need_dbias) {
   using namespace dense;
   if (M < 0 || N < 0 || K < 0) return -1;
-  return (need_dbias ? round256(4ll * MAX_SPANS * M) : 0) +
+  return (need_dbias ? round256(4ll * spans_of(N, M) * M) : 0) +
          (dz_apart(dC, lddc, N, act) ? packed_bytes(N, M) : 0) +
          (tma_lines(A, lda, K) ? 0 : packed_bytes(K, M)) +
          (tma_lines(B, ldb, N) ? 0 : packed_bytes(N, K));

@@ -66,48 +66,146 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 }
 
 // ---- activations --------------------------------------------------------------------
-// The logistic function by the fast exponential: relative error under 1e-6 for
-// |v| < 16, far below the half step of the 16-bit result (2^-9 and 2^-12).
-__device__ __forceinline__ float logistic(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// Evaluated on pairs: the packed f32x2 instructions take one issue slot for two
+// elements, and an epilogue's slots are what an activation costs (its power too).
+// ex2.approx.ftz and rcp.approx.ftz are documented to 2 ulp and 1 ulp; results
+// below the normal range become 0, which is below half a step of any output
+// they are added to or round to.
+using f2 = uint64_t;
+__device__ __forceinline__ f2 mk2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void un2(f2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f2 all2(float a) { return mk2(a, a); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ f2 ex2_2(f2 v) {
+  float a, b;
+  un2(v, a, b);
+  return mk2(ex2_fast(a), ex2_fast(b));
+}
+__device__ __forceinline__ f2 rcp_2(f2 v) {
+  float a, b;
+  un2(v, a, b);
+  return mk2(rcp_fast(a), rcp_fast(b));
+}
 
-constexpr float kSqrtHalf = 0.70710678118654752f;        // 1 / sqrt(2)
-constexpr float kInvSqrt2Pi = 0.39894228040143268f;      // 1 / sqrt(2 pi)
-constexpr float kGeluScale = 1.5957691216057308f;        // 2 sqrt(2 / pi)
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInvSqrt2Pi = 0.39894228040143268f;  // 1 / sqrt(2 pi)
+constexpr float kGeluScale = 1.5957691216057308f;    // 2 sqrt(2 / pi)
 constexpr float kGeluCube = 0.044715f;
 
-// 0.5 (1 + tanh(u)) is the logistic function of 2 u.
-template <int ACT>
-__device__ __forceinline__ float activate(float z) {
-  if (ACT == CTB_ACT_RELU) return z < 0.f ? 0.f : z;
-  if (ACT == CTB_ACT_SILU) return z * logistic(z);
-  if (ACT == CTB_ACT_GELU) return 0.5f * z * erfcf(-kSqrtHalf * z);
-  if (ACT == CTB_ACT_GELU_TANH) return z * logistic(kGeluScale * z * fmaf(kGeluCube * z, z, 1.f));
-  return z;
+// 1 / (1 + 2^v). 2^v = inf gives 0.
+__device__ __forceinline__ f2 logistic_ex2(f2 v) {
+  return rcp_2(add2(ex2_2(v), all2(1.f)));
 }
-template <int ACT>
-__device__ __forceinline__ float activate_slope(float z) {
-  if (ACT == CTB_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  if (ACT == CTB_ACT_SILU) {
-    const float s = logistic(z);
-    return s * fmaf(z, 1.f - s, 1.f);
-  }
-  if (ACT == CTB_ACT_GELU)
-    return fmaf(z * kInvSqrt2Pi, __expf(-0.5f * z * z), 0.5f * erfcf(-kSqrtHalf * z));
-  if (ACT == CTB_ACT_GELU_TANH) {
-    const float s = logistic(kGeluScale * z * fmaf(kGeluCube * z, z, 1.f));
-    return fmaf(z * s * (1.f - s), kGeluScale * fmaf(3.f * kGeluCube * z, z, 1.f), s);
-  }
-  return 1.f;
+
+// The upper tail of the normal distribution, Q(a) = 0.5 erfc(a / sqrt(2)), a >= 0,
+// and exp(-a^2 / 2) on the way: with t = 1 / (1 + 0.273 a), Q(a) exp(a^2 / 2) / t
+// is smooth in t over (0, 1]; this is its polynomial of degree 6 with the least
+// largest relative error (1.8e-6, by reweighted least squares on 4400 points
+// of [0, 40]). In 32 bits z * Phi(z) is within 4e-7 of the exact value for |z| <
+// 12. A call of erfcf instead made a 4096 x 4096 x 1024 layer take 115 us
+// against 51 us without an activation.
+__device__ __forceinline__ f2 normal_tail(f2 a, f2* density) {
+  const f2 e = ex2_2(mul2(mul2(a, a), all2(-0.5f * kLog2e)));
+  const f2 t = rcp_2(fma2(a, all2(0.273f), all2(1.f)));
+  f2 p = fma2(all2(-0.05735107883810997f), t, all2(0.14058725535869598f));
+  p = fma2(p, t, all2(-0.006268841680139303f));
+  p = fma2(p, t, all2(0.10854672640562057f));
+  p = fma2(p, t, all2(0.09625127166509628f));
+  p = fma2(p, t, all2(0.10933801531791687f));
+  p = fma2(p, t, all2(0.10889600962400436f));
+  *density = e;
+  return mul2(mul2(p, t), e);
 }
-// Chosen at run time, for code that the product does not wait on.
+
+// Both elements of a pair through the activation.
+template <int ACT>
+__device__ __forceinline__ void activate2(float& a, float& b) {
+  if (ACT == CTB_ACT_RELU) {
+    a = a < 0.f ? 0.f : a;
+    b = b < 0.f ? 0.f : b;
+  } else if (ACT == CTB_ACT_SILU) {
+    const f2 z = mk2(a, b);
+    un2(mul2(z, logistic_ex2(mul2(z, all2(-kLog2e)))), a, b);
+  } else if (ACT == CTB_ACT_GELU) {  // z Phi(z) = max(z, 0) - |z| Q(|z|)
+    f2 e;
+    const f2 q = normal_tail(mk2(fabsf(a), fabsf(b)), &e);
+    un2(fma2(mk2(-fabsf(a), -fabsf(b)), q, mk2(fmaxf(a, 0.f), fmaxf(b, 0.f))), a, b);
+  } else if (ACT == CTB_ACT_GELU_TANH) {  // 0.5 (1 + tanh(u)) is the logistic function of 2 u
+    const f2 z = mk2(a, b);
+    const f2 u = mul2(z, fma2(mul2(z, z), all2(-kLog2e * kGeluScale * kGeluCube),
+                              all2(-kLog2e * kGeluScale)));
+    un2(mul2(z, logistic_ex2(u)), a, b);
+  }
+}
+// Both elements of a pair replaced by the activation's slope there.
+template <int ACT>
+__device__ __forceinline__ void slope2(float& a, float& b) {
+  if (ACT == CTB_ACT_RELU) {
+    a = a > 0.f ? 1.f : 0.f;
+    b = b > 0.f ? 1.f : 0.f;
+  } else if (ACT == CTB_ACT_SILU) {  // s (1 + z (1 - s))
+    const f2 z = mk2(a, b);
+    const f2 s = logistic_ex2(mul2(z, all2(-kLog2e)));
+    un2(mul2(s, fma2(z, fma2(s, all2(-1.f), all2(1.f)), all2(1.f))), a, b);
+  } else if (ACT == CTB_ACT_GELU) {  // Phi(z) + z phi(z)
+    f2 e;
+    const f2 q = normal_tail(mk2(fabsf(a), fabsf(b)), &e);
+    const f2 d = mul2(mul2(mk2(a, b), all2(kInvSqrt2Pi)), e);
+    float qa, qb;
+    un2(q, qa, qb);
+    un2(add2(d, mk2(a > 0.f ? 1.f - qa : qa, b > 0.f ? 1.f - qb : qb)), a, b);
+  } else if (ACT == CTB_ACT_GELU_TANH) {  // s + z s (1 - s) * du/dz
+    const f2 z = mk2(a, b), zz = mul2(z, z);
+    const f2 s = logistic_ex2(mul2(z, fma2(zz, all2(-kLog2e * kGeluScale * kGeluCube),
+                                           all2(-kLog2e * kGeluScale))));
+    const f2 du = fma2(zz, all2(3.f * kGeluCube * kGeluScale), all2(kGeluScale));
+    const f2 w = mul2(mul2(z, s), fma2(s, all2(-1.f), all2(1.f)));
+    un2(fma2(w, du, s), a, b);
+  } else {
+    a = b = 1.f;
+  }
+}
+// Chosen at run time, one element: for code that nothing waits on.
 __device__ __forceinline__ float activate_any(float z, int act) {
+  float unused = 0.f;
   switch (act) {
-    case CTB_ACT_RELU: return activate<CTB_ACT_RELU>(z);
-    case CTB_ACT_GELU: return activate<CTB_ACT_GELU>(z);
-    case CTB_ACT_GELU_TANH: return activate<CTB_ACT_GELU_TANH>(z);
-    case CTB_ACT_SILU: return activate<CTB_ACT_SILU>(z);
-    default: return z;
+    case CTB_ACT_RELU: activate2<CTB_ACT_RELU>(z, unused); break;
+    case CTB_ACT_GELU: activate2<CTB_ACT_GELU>(z, unused); break;
+    case CTB_ACT_GELU_TANH: activate2<CTB_ACT_GELU_TANH>(z, unused); break;
+    case CTB_ACT_SILU: activate2<CTB_ACT_SILU>(z, unused); break;
+    default: break;
   }
+  return z;
 }
 
 }  // namespace dense

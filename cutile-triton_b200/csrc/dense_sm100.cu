@@ -46,7 +46,7 @@ struct Epilogue {
 template <typename T, int ACT>
 __device__ __forceinline__ void activate8(float (&z)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] = activate<ACT>(z[i]);
+  for (int i = 0; i < 8; i += 2) activate2<ACT>(z[i], z[i + 1]);
 }
 template <typename T>
 __device__ __forceinline__ void finish8(const Epilogue& e, int64_t r, int c, float (&z)[8]) {
@@ -350,8 +350,12 @@ __device__ __forceinline__ int box_at(int row, int piece) {
 template <typename T, int ACT>
 __device__ __forceinline__ void activate32(uint32_t (&v)[32]) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    v[j] = __float_as_uint(activate<ACT>(__uint_as_float(v[j])));
+  for (int j = 0; j < 32; j += 2) {
+    float x = __uint_as_float(v[j]), y = __uint_as_float(v[j + 1]);
+    activate2<ACT>(x, y);
+    v[j] = __float_as_uint(x);
+    v[j + 1] = __float_as_uint(y);
+  }
 }
 
 template <typename T, bool P_MN, bool Q_MN>

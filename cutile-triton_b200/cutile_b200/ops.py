@@ -329,14 +329,22 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+# The current stream's handle without building a torch Stream object (3 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call_on(device, name, *args):
     """One library call on the current stream of `device`, which need not be
     the current device."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+            rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 # ---- dense layer ------------------------------------------------------------------
