@@ -177,30 +177,37 @@ __global__ void __launch_bounds__(COMBINE_THREADS)
 #pragma unroll
     for (int e = 0; e < W; ++e) z[e] = 0.f;
     for (int c = lane * W; c < a.N; c += 32 * W) Run<T, W>::put(dy + c, z);
-  } else if (a.weights) {
-#pragma unroll 4
-    for (int c = lane * W; c < a.N; c += 32 * W) {
-      Run<T, W> rd, ry;
-      rd.load(d + c);
-      ry.load_once(y + c);
-      float fd[W], fy[W];
-      rd.get(fd);
-      ry.get(fy);
-#pragma unroll
-      for (int e = 0; e < W; ++e) {
-        dot = fmaf(fd[e], fy[e], dot);
-        fd[e] *= w;
-      }
-      Run<T, W>::put(dy + c, fd);
-    }
   } else {
-#pragma unroll 4
-    for (int c = lane * W; c < a.N; c += 32 * W) {
-      Run<T, W> rd;
-      rd.load(d + c);
-      float fd[W];
-      rd.get(fd);
-      Run<T, W>::put(dy + c, fd);
+    // FLIGHT runs of both rows are asked for before the first is used (the
+    // stores between them could alias, so the compiler would not).
+    constexpr int FLIGHT = 4;
+    for (int c0 = lane * W; c0 < a.N; c0 += FLIGHT * 32 * W) {
+      Run<T, W> rd[FLIGHT], ry[FLIGHT];
+#pragma unroll
+      for (int j = 0; j < FLIGHT; ++j) {
+        const int c = c0 + j * 32 * W;
+        if (c < a.N) {
+          rd[j].load(d + c);
+          if (a.weights) ry[j].load_once(y + c);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < FLIGHT; ++j) {
+        const int c = c0 + j * 32 * W;
+        if (c < a.N) {
+          float fd[W], fy[W];
+          rd[j].get(fd);
+          if (a.weights) {
+            ry[j].get(fy);
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+              dot = fmaf(fd[e], fy[e], dot);
+              fd[e] *= w;
+            }
+          }
+          Run<T, W>::put(dy + c, fd);
+        }
+      }
     }
   }
   if (a.weights) {

@@ -112,11 +112,12 @@ __device__ __forceinline__ S row_sum(S v) {
   return v;
 }
 
-// ---- order-preserving keys: 0 is "not available" -----------------------------------
-// Adding +0 first makes -0 and +0 the same key.
+// ---- order-preserving keys ----------------------------------------------------------
+// Adding +0 first makes -0 and +0 the same key. The key of -inf, and 0, stand
+// for "not available" (is_live); NaN has no key.
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t u = __float_as_uint(v + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return u ^ (uint32_t)((int32_t)u >> 31 | 0x80000000);
 }
 __device__ __forceinline__ uint64_t key_of(double v) {
   const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
@@ -125,6 +126,10 @@ __device__ __forceinline__ uint64_t key_of(double v) {
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
+constexpr uint32_t kNone32 = 0x007fffffu;              // key_of(-inf)
+constexpr uint64_t kNone64 = 0x000fffffffffffffull;
+__device__ __forceinline__ bool is_live(uint32_t k) { return k > kNone32; }
+__device__ __forceinline__ bool is_live(uint64_t k) { return k > kNone64; }
 template <typename S> struct KeyOf;
 template <> struct KeyOf<float> { using type = uint32_t; };
 template <> struct KeyOf<double> { using type = uint64_t; };
@@ -159,10 +164,25 @@ struct RouteArgs {
   float scale;
 };
 
+// The fast exponential and reciprocal: 2 and 1 ulp, results below the normal
+// range become 0.
+__device__ __forceinline__ float ex2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
 // Whether two choice values hi >= lo are too close for 32 bits to order them.
-// __expf is documented to 2 + 1.16 |d| ulp, so exp(d) carries at most 2.4e-7 +
-// 2e-7 |d| relative error with the rounding of d; the row's sum (its terms'
-// errors weighted, 8 levels of additions) at most 2e-6, the division 2.4e-7.
+// 2^(d log2 e) carries at most 2.4e-7 (ex2.approx) + 2e-7 |d| (the roundings of
+// d, of log2 e and of their product) relative error; the row's sum (its terms'
+// errors weighted, 8 levels of additions) at most 2e-6, reciprocal and product
+// 2.4e-7.
 // With a bias, the scores of a pair (or of two groups) of one row err by at
 // most 4e-6 together (softmax: they add up to at most 1; sigmoid: under 6e-7
 // each), and each addition by 2^-24 of the magnitude `mag`. Without one the
@@ -175,7 +195,8 @@ __device__ __forceinline__ bool too_close_unbiased(float hi, float lo) {
   return !(hi > 1e-30f && hi - lo > 2.f * hi * (4e-6f + 2.5e-7f * fabsf(__logf(hi))));
 }
 
-// Keys of the experts outside the best topk_groups groups become 0; returns
+// Keys of the experts outside the best topk_groups groups become 0 (c is -inf
+// where an expert is not available); returns
 // whether the choice between groups was too close for 32 bits. LANES == 32.
 template <typename S, int NV>
 __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV],
@@ -188,9 +209,8 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV]
     // Whole lanes per group: the two best of a lane's registers, then of neighbours.
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const S x = key[v] ? c[v] : none;
-      second = max(second, min(best, x));
-      best = max(best, x);
+      second = max(second, min(best, c[v]));
+      best = max(best, c[v]);
     }
     for (int o = 1; o < span; o <<= 1) {
       const S b = __shfl_xor_sync(FULL, best, o), s = __shfl_xor_sync(FULL, second, o);
@@ -206,7 +226,7 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV]
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int i = lane * NV + v;
-      if (i < a.E) row[i + (i >> 5)] = key[v] ? c[v] : none;
+      if (i < a.E) row[i + (i >> 5)] = c[v];
     }
     __syncwarp();
     if (lane < a.groups)
@@ -227,10 +247,21 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV]
   }
   const bool in = lane < a.groups && rank < a.topk_groups;
   const unsigned kept = __ballot_sync(FULL, in);
+  if (size % NV == 0) {  // a lane's experts share a group
+    if (lane * NV < a.E && !(kept >> (lane * NV / size) & 1u)) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int i = lane * NV + v;
-    if (i < a.E && !(kept >> (i / size) & 1u)) key[v] = 0;
+      for (int v = 0; v < NV; ++v) key[v] = 0;
+    }
+  } else {
+    int g = lane * NV / size, at = lane * NV - g * size;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (lane * NV + v < a.E && !(kept >> g & 1u)) key[v] = 0;
+      if (++at == size) {
+        at = 0;
+        ++g;
+      }
+    }
   }
   bool close = false;
   if (sizeof(S) == 4) {
@@ -248,52 +279,125 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV]
   return close;
 }
 
-// Writes the chosen experts to sel[0..topk); with `check`, returns whether two
-// neighbours in the order (the first one left out included) were too close.
+// The chosen experts of a row, largest first, and their keys; one place more
+// than topk where neighbours are to be checked.
+struct Chosen {
+  int id[ROUTE_MAX_TOPK + 1];
+  uint32_t key[ROUTE_MAX_TOPK + 1];  // of the 32-bit choice
+};
+
+// Fills row->id[0..rounds), -1 where no expert is left, and row->key for 32-bit keys.
+//
+// A whole warp's row with 32-bit keys: the rounds-th largest of the lanes' best
+// is a bound that at least `rounds` experts reach and few others do (12 of 256
+// for the best 8 of random scores); those candidates move to one lane each, and
+// a lane's rank among them is its place. 160 instructions for 8 of 256, against
+// 450 for choosing one after the other, which is left for rows with more than
+// 32 candidates, for narrower rows and for 64 bits. There a lane knows its two
+// best, so that it looks through its registers again only when it has been
+// chosen from twice.
 template <typename K, int LANES, int NV>
-__device__ __forceinline__ bool choose(const RouteArgs& a, K (&key)[NV], int* sel, bool check) {
+__device__ __forceinline__ void choose(K (&key)[NV], Chosen* row, uint64_t* cand, int rounds) {
   const int lane = threadIdx.x & 31, sub = lane % LANES, base = lane - sub;
-  bool close = false;
-  float before = INFINITY;
-  const int rounds = a.topk + (check ? 1 : 0);
-  K kb = 0;
-  int vb = 0;
-  auto rescan = [&] {
-    kb = key[0];
-    vb = 0;
+  if constexpr (LANES == 32 && sizeof(K) == 4) {
+    uint32_t t = key[0], bound = 0;
 #pragma unroll
-    for (int v = 1; v < NV; ++v)
-      if (key[v] > kb) {
-        kb = key[v];
-        vb = v;
-      }
-  };
-  rescan();
-  for (int j = 0; j < rounds; ++j) {
-    const K m = row_max_key<LANES>(kb);
-    const unsigned who = __ballot_sync(FULL, kb == m) >> base;
-    const int win = __ffs(LANES == 32 ? who : who & ((1u << (LANES & 31)) - 1u)) - 1;
-    if (check) {
-      const float v = m ? value_of((uint32_t)m) : -INFINITY;
-      if (m && j > 0) close |= too_close_biased(before, v, fabsf(before) + fabsf(v));
-      before = v;
+    for (int v = 1; v < NV; ++v) t = max(t, key[v]);
+    for (int j = 0; j < rounds; ++j) {
+      bound = __reduce_max_sync(FULL, t);
+      if (t == bound) t = 0;
     }
-    if (sub == win) {
-      if (j < a.topk) sel[j] = m ? sub * NV + vb : -1;
+    bound = max(bound, kNone32 + 1);
+    int total = 0, at[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const unsigned b = __ballot_sync(FULL, key[v] >= bound);
+      at[v] = total + __popc(b & ((1u << lane) - 1u));
+      total += __popc(b);
+    }
+    if (total <= 32) {
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        if (v == vb) key[v] = 0;
-      rescan();
+        if (key[v] >= bound) cand[at[v]] = (uint64_t)key[v] << 32 | (uint32_t)~(lane * NV + v);
+      __syncwarp();
+      const uint64_t mine = lane < total ? cand[lane] : 0;
+      int place = 0;
+      for (int i = 0; i < total; ++i) place += cand[i] > mine;
+      if (lane >= total) place = lane;  // places that no expert is left for
+      if (place < rounds) {
+        row->id[place] = mine ? (int)~(uint32_t)mine : -1;
+        row->key[place] = (uint32_t)(mine >> 32);
+      }
+      if (rounds > 32 && lane == 0) row->key[32] = 0;
+      __syncwarp();
+      return;
+    }
+  }
+  K k1 = 0, k2 = 0;
+  int v1 = 0, v2 = 0;
+  bool two = true;  // (k2, v2) is the second best still
+  auto scan = [&] {
+    k1 = k2 = 0;
+    v1 = v2 = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const K k = key[v];
+      if (k > k1) {
+        k2 = k1;
+        v2 = v1;
+        k1 = k;
+        v1 = v;
+      } else if (k > k2) {
+        k2 = k;
+        v2 = v;
+      }
+    }
+  };
+  scan();
+  unsigned taken = 0;
+  for (int j = 0; j < rounds; ++j) {
+    const K m = row_max_key<LANES>(k1);
+    const unsigned who = __ballot_sync(FULL, k1 == m) >> base;
+    const int win = __ffs(LANES == 32 ? who : who & ((1u << (LANES & 31)) - 1u)) - 1;
+    if (sub == win) {
+      row->id[j] = is_live(m) ? sub * NV + v1 : -1;
+      if (sizeof(K) == 4) row->key[j] = is_live(m) ? (uint32_t)m : 0u;
+      taken |= 1u << v1;
+      if (two) {
+        k1 = k2;
+        v1 = v2;
+        two = false;
+      } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+          if (taken >> v & 1u) key[v] = 0;
+        scan();
+        two = true;
+      }
     }
   }
   __syncwarp();
+}
+
+// Whether two neighbours in the order (the first one left out included) are
+// too close.
+template <int LANES>
+__device__ __forceinline__ bool neighbours_close(const Chosen* row, int topk) {
+  bool close = false;
+  for (int j = threadIdx.x % LANES; j < topk; j += LANES) {
+    const uint32_t hi = row->key[j], lo = row->key[j + 1];
+    if (lo) {
+      const float x = value_of(hi), y = value_of(lo);
+      close |= too_close_biased(x, y, fabsf(x) + fabsf(y));
+    }
+  }
   return close;
 }
 
 // The same row ranked in 64 bits.
 template <typename T, int LANES, int NV, bool GROUPED>
 __device__ __noinline__ void choose_exact(const RouteArgs& a, const T* __restrict__ x, int i0,
-                                          bool in_range, int* sel, double* row) {
+                                          bool in_range, Chosen* sel, double* row) {
   double c[NV];
   uint64_t key[NV];
   double top = -INFINITY;
@@ -318,11 +422,11 @@ __device__ __noinline__ void choose_exact(const RouteArgs& a, const T* __restric
     const double xv = c[v];
     const double s = a.sigmoid ? 1.0 / (1.0 + exp(-xv)) : exp(xv - top) / total;
     c[v] = a.bias && i0 + v < a.E ? s + (double)a.bias[i0 + v] : s;
-    const bool live = xv > -INFINITY && c[v] > -INFINITY;
-    key[v] = live ? key_of(a.bias ? c[v] : xv) : 0;
+    if (!(xv > -INFINITY && c[v] > -INFINITY)) c[v] = -INFINITY;
+    key[v] = key_of(a.bias || !(c[v] > -INFINITY) ? c[v] : xv);
   }
   if (GROUPED) keep_groups<double, NV>(a, c, key, row);
-  choose<uint64_t, LANES, NV>(a, key, sel, false);
+  choose<uint64_t, LANES, NV>(key, sel, nullptr, a.topk);
 }
 
 template <typename T, int LANES, int NV, bool VEC, bool GROUPED>
@@ -330,14 +434,15 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __res
                                                                   const RouteArgs a) {
   constexpr int ROWS = ROUTE_THREADS / LANES;
   constexpr int SLOTS = ROUTE_MAX_TOPK / LANES;  // places of a row per lane
-  __shared__ int sel_all[ROWS][ROUTE_MAX_TOPK];
+  __shared__ Chosen sel_all[ROWS];
+  __shared__ uint64_t cand[LANES == 32 ? ROUTE_THREADS / 32 : 1][LANES == 32 ? 32 : 1];
   __shared__ double scratch[GROUPED ? ROUTE_THREADS / 32 : 1]
                            [GROUPED ? ROUTE_MAX_EXPERTS + ROUTE_MAX_EXPERTS / 32 : 1];
   const int lane = threadIdx.x & 31, sub = lane % LANES, r = threadIdx.x / LANES;
   const int64_t t = (int64_t)blockIdx.x * ROWS + r;
   const bool in_range = t < a.T;
   const T* xr = x + (in_range ? t : 0) * a.ldx;
-  int* sel = sel_all[r];
+  Chosen* sel = &sel_all[r];
   const int i0 = sub * NV;
 
   float xv[NV];
@@ -345,7 +450,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __res
   float top = -INFINITY;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    if (isnan(xv[v])) xv[v] = -INFINITY;
+    xv[v] = fmaxf(xv[v], -INFINITY);  // NaN becomes -inf
     top = fmaxf(top, xv[v]);
   }
   // Softmax over the row, where the choice or the weights need it.
@@ -356,26 +461,30 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __res
     if (top == -INFINITY) top = 0.f;
     total = 0.f;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) total += __expf(xv[v] - top);
+    for (int v = 0; v < NV; ++v) total += ex2_fast(kLog2e * (xv[v] - top));
     total = row_sum<LANES>(total);
   }
+  const float scale_of = rcp_fast(total);
   float c[NV];
   uint32_t key[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     c[v] = xv[v];
     if (scores) {
-      const float s = a.sigmoid ? __fdividef(1.f, 1.f + __expf(-xv[v]))
-                                : __fdividef(__expf(xv[v] - top), total);
-      c[v] = a.bias && i0 + v < a.E ? s + a.bias[i0 + v] : s;
+      const float s = a.sigmoid ? rcp_fast(1.f + ex2_fast(-kLog2e * xv[v]))
+                                : ex2_fast(kLog2e * (xv[v] - top)) * scale_of;
+      c[v] = a.bias && i0 + v < a.E ? fmaxf(s + a.bias[i0 + v], -INFINITY) : s;
+      if (xv[v] == -INFINITY) c[v] = -INFINITY;
     }
-    const bool live = xv[v] > -INFINITY && c[v] > -INFINITY;
-    key[v] = live ? key_of(a.bias ? c[v] : xv[v]) : 0u;
+    key[v] = key_of(a.bias ? c[v] : xv[v]);
   }
   bool close = false;
   double* row = scratch[GROUPED ? threadIdx.x / 32 : 0];
   if (GROUPED) close = keep_groups<float, NV>(a, c, key, reinterpret_cast<float*>(row));
-  close |= choose<uint32_t, LANES, NV>(a, key, sel, a.bias != nullptr);
+  const bool check = a.bias != nullptr;
+  choose<uint32_t, LANES, NV>(key, sel, cand[LANES == 32 ? threadIdx.x / 32 : 0],
+                              a.topk + (check ? 1 : 0));
+  if (check) close |= neighbours_close<LANES>(sel, a.topk);
   if (__any_sync(FULL, close && in_range))
     choose_exact<T, LANES, NV, GROUPED>(a, xr, i0, in_range, sel, row);
 
@@ -386,7 +495,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __res
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
     const int j = sub + i * LANES;
-    id[i] = in_range && j < a.topk ? sel[j] : -1;
+    id[i] = in_range && j < a.topk ? sel->id[j] : -1;
     xs[i] = id[i] >= 0 ? to_float(xr[id[i]]) : -INFINITY;
     m = fmaxf(m, xs[i]);
   }
