@@ -15,7 +15,7 @@ namespace dense {
 
 // dense_sm100.cu
 template <typename T>
-int product_sm100(const Product& p, cudaStream_t st);
+int product_sm100(const Product& p, int sms, cudaStream_t st);
 
 namespace {
 
@@ -85,7 +85,7 @@ int pack_operand(const void** p, int64_t* ld, int64_t lines, int64_t len, uint8_
 
 template <typename T>
 int product(const Product& p, int sms, cudaStream_t st) {
-  if (p.depth > 0) return product_sm100<T>(p, st);
+  if (p.depth > 0) return product_sm100<T>(p, sms, st);
   const int64_t grid = std::min<int64_t>(((int64_t)p.rows * p.cols + 255) / 256, 16ll * sms);
   product_empty_kernel<T><<<(unsigned)grid, 256, 0, st>>>(p);
   return launch_status("product_empty_kernel");

@@ -710,12 +710,15 @@ int split_attrs() {
   return rc;
 }
 
-int device_setup() {
+// Kernel attributes of the current device, once per context; `pairs` receives the
+// CTA pairs that are resident at once.
+int device_setup(int* pairs_out) {
   int dev = 0;
   CTB_CUDA_CHECK(cudaGetDevice(&dev));
   std::lock_guard<std::mutex> lk(g_dense_mu);
   unsigned long long ctx = 0;
   if (int rc = current_context_id(&ctx)) return rc;
+  *pairs_out = dev < 64 ? g_dense_pairs[dev] : 0;
   if (dev < 64 && g_dense_ctx[dev] == ctx) return CTB_OK;
   if (int rc = split_attrs<__half>()) return rc;
   if (int rc = split_attrs<__nv_bfloat16>()) return rc;
@@ -730,6 +733,7 @@ int device_setup() {
     g_dense_pairs[dev] = pairs;
     g_dense_ctx[dev] = ctx;
   }
+  *pairs_out = pairs;
   return CTB_OK;
 }
 
@@ -821,10 +825,9 @@ int pair_launch(const Product& p, const Epilogue& e, int pairs, cudaStream_t st)
 // The product on the tensor cores. Operands start on 16-byte boundaries, their
 // leading dimensions are multiples of 8 (or they have one line only); depth > 0.
 template <typename T>
-int product_sm100(const Product& p0, cudaStream_t st) {
-  DeviceProps pr;
-  if (int rc = current_props(&pr)) return rc;
-  if (int rc = device_setup()) return rc;
+int product_sm100(const Product& p0, int sms, cudaStream_t st) {
+  int pairs = 0;
+  if (int rc = device_setup(&pairs)) return rc;
   Product p = p0;
   // The distance between lines does not matter where there is one: any that TMA takes.
   if ((p.p_mn ? p.depth : p.rows) == 1) p.ldp = ((p.p_mn ? p.rows : p.depth) + 7) / 8 * 8;
@@ -843,10 +846,6 @@ int product_sm100(const Product& p0, cudaStream_t st) {
   e.bias_f32 = p.bias_f32;
   e.vec = rows16(p.D, p.ldd, p.rows) && (!p.Z || rows16(p.Z, p.ldz, p.rows)) &&
           (!p.R || rows16(p.R, p.ldr, p.rows));
-  const int sms = pr.sm_count;
-  int dev = 0;
-  CTB_CUDA_CHECK(cudaGetDevice(&dev));
-  const int pairs = dev < 64 ? g_dense_pairs[dev] : 0;
   const int64_t pair_tiles = (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
   const int min_tiles = pair_min_tiles() >= 0 ? pair_min_tiles() : pairs / 2;
   if (pairs > 0 && pair_tiles >= std::max(1, min_tiles)) {
@@ -869,8 +868,8 @@ int product_sm100(const Product& p0, cudaStream_t st) {
   if (p.rows <= 64) return split_launch<T, false, false, 64>(p, e, sms, st);
   return split_launch<T, false, false, 128>(p, e, sms, st);
 }
-template int product_sm100<__half>(const Product&, cudaStream_t);
-template int product_sm100<__nv_bfloat16>(const Product&, cudaStream_t);
+template int product_sm100<__half>(const Product&, int, cudaStream_t);
+template int product_sm100<__nv_bfloat16>(const Product&, int, cudaStream_t);
 
 }  // namespace dense
 

@@ -289,34 +289,46 @@ def _need(ok, code, msg):
         raise _lib.B200Error(code, msg)
 
 
+def _need_rows(t, what):
+    """A 2-D CUDA tensor with contiguous rows: what a call's first matrix must
+    be, whose shape, dtype and device the others are held to."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise _lib.B200Error(-1, f"{what}: expected CUDA tensors")
+    if t.dim() != 2:
+        raise _lib.B200Error(-3, f"{what}: expected a matrix, got {t.dim()} dimensions")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise _lib.B200Error(-4, f"{what}: rows must be contiguous")
+
+
 def _need_matrix(t, rows, cols, dtype, device, what):
     """A (rows, cols) CUDA matrix of `dtype` on `device` with contiguous rows."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        raise _lib.B200Error(-1, f"{what}: expected a CUDA tensor")
-    if t.device != device:
-        raise _lib.B200Error(-1, f"{what}: on {t.device}, the other tensors are on {device}")
+    if not (isinstance(t, torch.Tensor) and t.device == device):
+        at = t.device if isinstance(t, torch.Tensor) else type(t).__name__
+        raise _lib.B200Error(-1, f"{what}: expected a CUDA tensor on {device}, got {at}")
     if t.dtype != dtype:
         raise _lib.B200Error(-2, f"{what}: expected {dtype}, got {t.dtype}")
     if t.shape != (rows, cols):
         raise _lib.B200Error(-3, f"{what}: expected shape ({rows}, {cols}), got {tuple(t.shape)}")
-    if cols > 1 and t.stride(1) != 1:
+    if t.stride(1) != 1 and cols > 1:
         raise _lib.B200Error(-4, f"{what}: rows must be contiguous")
-    return t
 
 
 def _need_packed(t, shape, dtype, device, what):
     """A contiguous CUDA tensor of exactly this shape and dtype."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        raise _lib.B200Error(-1, f"{what}: expected a CUDA tensor")
-    if t.device != device:
-        raise _lib.B200Error(-1, f"{what}: on {t.device}, the other tensors are on {device}")
+    if not (isinstance(t, torch.Tensor) and t.device == device):
+        at = t.device if isinstance(t, torch.Tensor) else type(t).__name__
+        raise _lib.B200Error(-1, f"{what}: expected a CUDA tensor on {device}, got {at}")
     if t.dtype != dtype:
         raise _lib.B200Error(-2, f"{what}: expected {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise _lib.B200Error(-3, f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise _lib.B200Error(-4, f"{what}: must be contiguous")
-    return t
+
+
+def _new_matrix(rows, cols, dtype, device):
+    # empty_strided takes 1.6 us, empty with a shape 2.4
+    return torch.empty_strided((rows, cols), (cols if cols > 0 else 1, 1), dtype=dtype, device=device)
 
 
 def _ld(t):
@@ -354,15 +366,19 @@ _ACTS = {"none": _lib.CTB_ACT_NONE, "relu": _lib.CTB_ACT_RELU, "gelu": _lib.CTB_
 
 def _dense_operands(k, A_t, B_t, act):
     """Checks the weight (K, M) and the activations (N, K) -> (M, N, K, dtype, device)."""
-    _need_cuda(A_t, B_t)
-    _need(A_t.dim() == 2 and B_t.dim() == 2, -3, f"{k}: A_t must be (K, M), B_t (N, K)")
-    _need(act in _ACTS, -1, f"{k}: unknown activation {act!r}")
+    _need_rows(A_t, k)
+    _need_rows(B_t, k)
+    if act not in _ACTS:
+        raise _lib.B200Error(-1, f"{k}: unknown activation {act!r}")
     dt, dev = A_t.dtype, A_t.device
-    _need(dt in (torch.float16, torch.bfloat16), -2, f"{k}: float16 or bfloat16, got {dt}")
+    if (dt is not torch.float16 and dt is not torch.bfloat16) or B_t.dtype is not dt:
+        raise _lib.B200Error(-2, f"{k}: both float16 or both bfloat16, got {dt} and {B_t.dtype}")
     K, M = A_t.shape
-    N = B_t.shape[0]
-    _need_matrix(A_t, K, M, dt, dev, f"{k}: A_t")
-    _need_matrix(B_t, N, K, dt, dev, f"{k}: B_t")
+    N, kb = B_t.shape
+    if kb != K:
+        raise _lib.B200Error(-3, f"{k}: A_t must be (K, M), B_t (N, K)")
+    if B_t.device != dev:
+        raise _lib.B200Error(-1, f"{k}: A_t is on {dev}, B_t on {B_t.device}")
     return M, N, K, dt, dev
 
 
@@ -389,13 +405,15 @@ def dense(A_t, B_t, bias=None, act="none", residual=None, out=None, preact=None)
     if preact is not None:
         _need_matrix(preact, N, M, dt, dev, "dense: preact")
     if out is None:
-        out = torch.empty((N, M), dtype=dt, device=dev)
+        out = _new_matrix(N, M, dt, dev)
     else:
         _need_matrix(out, N, M, dt, dev, "dense: out")
     lda, ldb = _ld(A_t), _ld(B_t)
     pa, pb = A_t.data_ptr(), B_t.data_ptr()
-    nws = _lib.load().ctb_dense_fwd_workspace_bytes(pa, pb, M, N, K, lda, ldb)
-    ws = _workspace(nws, dev)
+    nws, ws = 0, None
+    if (pa | pb) & 15 or (lda | ldb) & 7:
+        nws = _lib.load().ctb_dense_fwd_workspace_bytes(pa, pb, M, N, K, lda, ldb)
+        ws = _workspace(nws, dev)
     _call_on(dev, "ctb_dense_fwd", _DT[dt], pa, pb, _ptr(bias),
              0 if bias is None else _DT[bias.dtype], _ptr(residual), _ptr(preact), out.data_ptr(),
              M, N, K, lda, ldb, 0 if residual is None else _ld(residual),
@@ -418,13 +436,13 @@ def dense_bwd(dC_t, A_t, B_t, act="none", preact=None, dA_t=None, dB_t=None, dbi
     if not need_dA:
         dA_t = None
     elif dA_t is None:
-        dA_t = torch.empty((K, M), dtype=dt, device=dev)
+        dA_t = _new_matrix(K, M, dt, dev)
     else:
         _need_matrix(dA_t, K, M, dt, dev, "dense_bwd: dA_t")
     if not need_dB:
         dB_t = None
     elif dB_t is None:
-        dB_t = torch.empty((N, K), dtype=dt, device=dev)
+        dB_t = _new_matrix(N, K, dt, dev)
     else:
         _need_matrix(dB_t, N, K, dt, dev, "dense_bwd: dB_t")
     if not need_dbias:
@@ -463,25 +481,23 @@ def moe_route(logits, topk, score="softmax", bias=None, groups=1, topk_groups=No
     the sum of the chosen s. An expert with a logit or c of -inf or NaN is not
     available; places no expert is left for get id -1 and weight 0 (a row of
     -inf, a padding token, goes to no expert). E <= 256, topk <= 32."""
-    _need_cuda(logits)
-    _need(logits.dim() == 2, -3, "moe_route: logits must be (T, E)")
+    _need_rows(logits, "moe_route: logits")
     _need(isinstance(topk, int) and topk >= 1, -3, "moe_route: topk must be positive")
-    _need(score in _SCORES, -1, f"moe_route: unknown score {score!r}")
-    _need(logits.dtype in _DT, -2, f"moe_route: unsupported dtype {logits.dtype}")
+    if score not in _SCORES:
+        raise _lib.B200Error(-1, f"moe_route: unknown score {score!r}")
     T, E = logits.shape
     dev = logits.device
-    _need_matrix(logits, T, E, logits.dtype, dev, "moe_route: logits")
     if bias is not None:
         _need_packed(bias, (E,), torch.float32, dev, "moe_route: bias")
     if weights is None:
-        weights = torch.empty((T, topk), dtype=torch.float32, device=dev)
+        weights = _new_matrix(T, topk, torch.float32, dev)
     else:
         _need_packed(weights, (T, topk), torch.float32, dev, "moe_route: weights")
     if ids is None:
-        ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
+        ids = _new_matrix(T, topk, torch.int32, dev)
     else:
         _need_packed(ids, (T, topk), torch.int32, dev, "moe_route: ids")
-    _call_on(dev, "ctb_moe_route", _DT[logits.dtype], logits.data_ptr(), _ptr(bias),
+    _call_on(dev, "ctb_moe_route", _DT.get(logits.dtype, 0), logits.data_ptr(), _ptr(bias),
              weights.data_ptr(), ids.data_ptr(), T, E, topk, _ld(logits), _SCORES[score], groups,
              groups if topk_groups is None else topk_groups, group_top, 1 if renorm else 0, scale)
     return weights, ids
@@ -491,36 +507,34 @@ def moe_route_bwd(dweights, logits, ids, score="softmax", renorm=True, scale=1.0
     """Gradient of :func:`moe_route`'s weights: dlogits (T, E, dtype of the
     logits) from dweights (T, topk) and the ids of the forward call. The
     choice and its bias have no gradient."""
-    _need_cuda(dweights, logits, ids)
-    _need(logits.dim() == 2 and ids.dim() == 2, -3,
-          "moe_route_bwd: logits must be (T, E), ids (T, topk)")
-    _need(score in _SCORES, -1, f"moe_route_bwd: unknown score {score!r}")
-    _need(logits.dtype in _DT, -2, f"moe_route_bwd: unsupported dtype {logits.dtype}")
+    _need_rows(logits, "moe_route_bwd: logits")
+    _need_rows(ids, "moe_route_bwd: ids")
+    if score not in _SCORES:
+        raise _lib.B200Error(-1, f"moe_route_bwd: unknown score {score!r}")
     T, E = logits.shape
     topk = ids.shape[1]
     dev = logits.device
-    _need_matrix(logits, T, E, logits.dtype, dev, "moe_route_bwd: logits")
     _need_packed(ids, (T, topk), torch.int32, dev, "moe_route_bwd: ids")
     _need_packed(dweights, (T, topk), torch.float32, dev, "moe_route_bwd: dweights")
     if dlogits is None:
-        dlogits = torch.empty((T, E), dtype=logits.dtype, device=dev)
+        dlogits = _new_matrix(T, E, logits.dtype, dev)
     else:
         _need_matrix(dlogits, T, E, logits.dtype, dev, "moe_route_bwd: dlogits")
-    _call_on(dev, "ctb_moe_route_bwd", _DT[logits.dtype], dweights.data_ptr(), logits.data_ptr(),
+    _call_on(dev, "ctb_moe_route_bwd", _DT.get(logits.dtype, 0), dweights.data_ptr(), logits.data_ptr(),
              ids.data_ptr(), dlogits.data_ptr(), T, E, topk, _ld(logits), _ld(dlogits),
              _SCORES[score], 1 if renorm else 0, scale)
     return dlogits
 
 
 def _combine_args(k, rows, topk, weights, ids, num_experts, dev):
-    _need(isinstance(topk, int) and topk >= 1 and rows % topk == 0, -3,
-          f"{k}: y must have T * topk rows")
+    if not (isinstance(topk, int) and topk >= 1 and rows % topk == 0):
+        raise _lib.B200Error(-3, f"{k}: y must have T * topk rows")
     T = rows // topk
     if weights is not None:
-        _need_packed(weights, (T, topk), torch.float32, dev, f"{k}: weights")
+        _need_packed(weights, (T, topk), torch.float32, dev, "weights")
     if ids is not None:
-        _need_packed(ids, (T, topk), torch.int32, dev, f"{k}: ids")
-        _need(num_experts is not None, -1, f"{k}: ids need num_experts")
+        _need_packed(ids, (T, topk), torch.int32, dev, "ids")
+        _need(num_experts is not None, -1, "ids need num_experts")
     return T, int(num_experts) if ids is not None else 0
 
 
@@ -532,20 +546,17 @@ def moe_combine(y, topk, weights=None, ids=None, num_experts=None, residual=None
     `ids` (T, topk) int32 and `num_experts`, slots with an id outside
     [0, num_experts) are skipped: no expert wrote their rows, which are not
     read. `out` may be `residual`."""
-    _need_cuda(y)
-    _need(y.dim() == 2, -3, "moe_combine: y must be (T * topk, N)")
-    _need(y.dtype in _DT, -2, f"moe_combine: unsupported dtype {y.dtype}")
+    _need_rows(y, "moe_combine: y")
     rows, N = y.shape
     dev = y.device
-    _need_matrix(y, rows, N, y.dtype, dev, "moe_combine: y")
     T, E = _combine_args("moe_combine", rows, topk, weights, ids, num_experts, dev)
     if residual is not None:
         _need_matrix(residual, T, N, y.dtype, dev, "moe_combine: residual")
     if out is None:
-        out = torch.empty((T, N), dtype=y.dtype, device=dev)
+        out = _new_matrix(T, N, y.dtype, dev)
     else:
         _need_matrix(out, T, N, y.dtype, dev, "moe_combine: out")
-    _call_on(dev, "ctb_moe_combine", _DT[y.dtype], y.data_ptr(), _ptr(weights), _ptr(ids),
+    _call_on(dev, "ctb_moe_combine", _DT.get(y.dtype, 0), y.data_ptr(), _ptr(weights), _ptr(ids),
              _ptr(residual), out.data_ptr(), T, topk, N, E, _ld(y),
              0 if residual is None else _ld(residual), _ld(out))
     return out
@@ -556,14 +567,11 @@ def moe_combine_bwd(dout, y, topk, weights=None, ids=None, num_experts=None, dy=
     """Gradients of :func:`moe_combine` -> (dy (T * topk, N), dweights (T, topk)
     float32, None without weights). Skipped slots get zeros. The gradient of
     the residual is `dout`. Without weights `y` is not used and may be None."""
-    _need_cuda(dout)
-    _need(dout.dim() == 2, -3, "moe_combine_bwd: dout must be (T, N)")
-    _need(dout.dtype in _DT, -2, f"moe_combine_bwd: unsupported dtype {dout.dtype}")
+    _need_rows(dout, "moe_combine_bwd: dout")
     T, N = dout.shape
     dev = dout.device
     _need(isinstance(topk, int) and topk >= 1, -3, "moe_combine_bwd: topk must be positive")
     rows = T * topk
-    _need_matrix(dout, T, N, dout.dtype, dev, "moe_combine_bwd: dout")
     T, E = _combine_args("moe_combine_bwd", rows, topk, weights, ids, num_experts, dev)
     if weights is None:
         _need(dweights is None, -1, "moe_combine_bwd: dweights without weights")
@@ -571,14 +579,14 @@ def moe_combine_bwd(dout, y, topk, weights=None, ids=None, num_experts=None, dy=
     else:
         _need_matrix(y, rows, N, dout.dtype, dev, "moe_combine_bwd: y")
         if dweights is None:
-            dweights = torch.empty((T, topk), dtype=torch.float32, device=dev)
+            dweights = _new_matrix(T, topk, torch.float32, dev)
         else:
             _need_packed(dweights, (T, topk), torch.float32, dev, "moe_combine_bwd: dweights")
     if dy is None:
-        dy = torch.empty((rows, N), dtype=dout.dtype, device=dev)
+        dy = _new_matrix(rows, N, dout.dtype, dev)
     else:
         _need_matrix(dy, rows, N, dout.dtype, dev, "moe_combine_bwd: dy")
-    _call_on(dev, "ctb_moe_combine_bwd", _DT[dout.dtype], dout.data_ptr(), _ptr(y), _ptr(weights),
+    _call_on(dev, "ctb_moe_combine_bwd", _DT.get(dout.dtype, 0), dout.data_ptr(), _ptr(y), _ptr(weights),
              _ptr(ids), dy.data_ptr(), _ptr(dweights), T, topk, N, E, _ld(dout),
              0 if y is None else _ld(y), _ld(dy))
     return dy, dweights
