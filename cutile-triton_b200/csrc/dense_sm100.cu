@@ -748,21 +748,76 @@ int operand_map(CUtensorMap* m, const void* base, int64_t ld, bool mn, int exten
   return encode_tmap(m, Format<T>::map, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// CTB_DENSE_PAIR_TILES=n: the pair kernel from n tiles on (a measuring aid).
-static int pair_min_tiles() {
-  static const int n = [] {
-    const char* v = getenv("CTB_DENSE_PAIR_TILES");
-    return v ? atoi(v) : -1;
-  }();
-  return n;
-}
-
 static bool rows16(const void* p, int64_t ld, int rows) {
   return aligned16(p) && (ld % 8 == 0 || rows <= 1);
 }
 
+// ---- which kernel, tile and split ------------------------------------------------------
+// A model of the two kernels' times in microseconds, fitted to 50 products of 1
+// to 512 rows and 512 to 14336 columns and k (on average 3% off the best tile and
+// split measured). A split CTA takes its k-blocks at 60 GB/s when alone on its SM,
+// two together at 100; 256 CTAs of clusters are sure to be resident at once, 296
+// single ones. A pair takes 0.31 us a k-block.
+struct Plan {
+  int BN, S;  // BN = 0: the pair kernel
+};
+
+static double split_us(const Product& p, int BN, int S, int sms, double hbm_us) {
+  const int64_t tiles = (int64_t)((p.cols + SP_COLS - 1) / SP_COLS) * ((p.rows + BN - 1) / BN);
+  const int64_t ctas = tiles * S;
+  const int kb = (p.depth + BK - 1) / BK, per = (kb + S - 1) / S;
+  const double waves = (double)((ctas + 2 * sms - 1) / (2 * sms));
+  const double both = ctas > sms ? 2 : 1;
+  const double bytes = (double)per * sp_stage_bytes(BN);
+  const double load = waves * std::max(bytes / 60e3, both * bytes / 100e3);
+  return 4 + std::max(load, hbm_us) + waves * both * BN * 0.03 + (S > 1 ? 0.5 : 0) + 0.2 * S;
+}
+static double pair_us(const Product& p, int pairs, double hbm_us) {
+  const int64_t tiles = (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
+  const int kb = (p.depth + BK - 1) / BK;
+  const double waves = (double)((tiles + pairs - 1) / pairs);
+  return 5.5 + std::max(waves * (1 + 0.31 * kb), hbm_us);
+}
+
+// CTB_DENSE_PAIR=0 never takes the pair kernel, =1 whenever a pair can be resident.
+static int pair_mode() {
+  static const int mode = [] {
+    const char* v = getenv("CTB_DENSE_PAIR");
+    return v ? (v[0] == '1' ? 1 : 0) : -1;
+  }();
+  return mode;
+}
+
+static Plan choose_plan(const Product& p, int sms, int pairs) {
+  const double out = 1 + (p.Z ? 1 : 0) + (p.R ? 1 : 0);
+  const double hbm_us = ((double)p.cols * p.depth + (double)p.rows * p.depth +
+                         out * (double)p.rows * p.cols) * 2 / 6e6;
+  Plan best = {0, 1};
+  double us = pairs > 0 ? pair_us(p, pairs, hbm_us) : 1e30;
+  const int mode = pair_mode();
+  if (mode == 1 && pairs > 0) return best;
+  if (mode == 0) us = 1e30;
+  const int64_t tiles_c = (p.cols + SP_COLS - 1) / SP_COLS;
+  const int kb = (p.depth + BK - 1) / BK;
+  for (int BN = p.p_mn ? 64 : 16; BN <= 128; BN *= 2) {
+    const int64_t tiles_r = (p.rows + BN - 1) / BN;
+    if (tiles_r > 65535 && !(BN == 128 && us >= 1e30)) continue;  // the grid's y
+    for (int S = 1; S <= 8; ++S) {
+      if (S > 1 && (S > kb / 2 || tiles_c * tiles_r * S > 256)) break;
+      if (S == 5 || S == 7) continue;
+      const double t = split_us(p, BN, S, sms, hbm_us);
+      if (t < us) {
+        us = t;
+        best = {BN, S};
+      }
+    }
+    if (BN >= p.rows) break;  // a wider tile has no more rows
+  }
+  return best;
+}
+
 template <typename T, bool Q_MN, bool P_MN, int BN>
-int split_launch(const Product& p, const Epilogue& e, int sms, cudaStream_t st) {
+int split_launch(const Product& p, const Epilogue& e, int S, cudaStream_t st) {
   CUtensorMap tmQ, tmP;
   if (int rc = operand_map<T>(&tmQ, p.Q, p.ldq, Q_MN, p.cols, p.depth, SP_COLS)) return rc;
   if (int rc = operand_map<T>(&tmP, p.P, p.ldp, P_MN, p.rows, p.depth, BN)) return rc;
@@ -771,9 +826,6 @@ int split_launch(const Product& p, const Epilogue& e, int sms, cudaStream_t st) 
   a.num_kb = (p.depth + BK - 1) / BK;
   const int64_t tiles_c = (p.cols + SP_COLS - 1) / SP_COLS, tiles_r = ((int64_t)p.rows + BN - 1) / BN;
   if (tiles_r > 65535) return set_error(CTB_ERR_SHAPE, "dense: too many rows");
-  // As many CTAs per tile as fill two per SM once, with 2 k-blocks each at least.
-  int S = (int)std::max<int64_t>(1, std::min<int64_t>(8, 2ll * sms / (tiles_c * tiles_r)));
-  S = std::max(1, std::min(S, a.num_kb / 2));
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr;
   cluster_config(&cfg, &attr, dim3((unsigned)(tiles_c * S), (unsigned)tiles_r, 1), SP_THREADS,
@@ -846,27 +898,26 @@ int product_sm100(const Product& p0, int sms, cudaStream_t st) {
   e.bias_f32 = p.bias_f32;
   e.vec = rows16(p.D, p.ldd, p.rows) && (!p.Z || rows16(p.Z, p.ldz, p.rows)) &&
           (!p.R || rows16(p.R, p.ldr, p.rows));
-  const int64_t pair_tiles = (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
-  const int min_tiles = pair_min_tiles() >= 0 ? pair_min_tiles() : pairs / 2;
-  if (pairs > 0 && pair_tiles >= std::max(1, min_tiles)) {
+  const Plan plan = choose_plan(p, sms, pairs);
+  if (plan.BN == 0) {
     if (p.p_mn) return pair_launch<T, true, true>(p, e, pairs, st);
     if (p.q_mn) return pair_launch<T, false, true>(p, e, pairs, st);
     return pair_launch<T, false, false>(p, e, pairs, st);
   }
   if (p.p_mn) {
-    if (p.rows <= 64) return split_launch<T, true, true, 64>(p, e, sms, st);
-    return split_launch<T, true, true, 128>(p, e, sms, st);
+    if (plan.BN == 64) return split_launch<T, true, true, 64>(p, e, plan.S, st);
+    return split_launch<T, true, true, 128>(p, e, plan.S, st);
   }
   if (p.q_mn) {
-    if (p.rows <= 16) return split_launch<T, true, false, 16>(p, e, sms, st);
-    if (p.rows <= 32) return split_launch<T, true, false, 32>(p, e, sms, st);
-    if (p.rows <= 64) return split_launch<T, true, false, 64>(p, e, sms, st);
-    return split_launch<T, true, false, 128>(p, e, sms, st);
+    if (plan.BN == 16) return split_launch<T, true, false, 16>(p, e, plan.S, st);
+    if (plan.BN == 32) return split_launch<T, true, false, 32>(p, e, plan.S, st);
+    if (plan.BN == 64) return split_launch<T, true, false, 64>(p, e, plan.S, st);
+    return split_launch<T, true, false, 128>(p, e, plan.S, st);
   }
-  if (p.rows <= 16) return split_launch<T, false, false, 16>(p, e, sms, st);
-  if (p.rows <= 32) return split_launch<T, false, false, 32>(p, e, sms, st);
-  if (p.rows <= 64) return split_launch<T, false, false, 64>(p, e, sms, st);
-  return split_launch<T, false, false, 128>(p, e, sms, st);
+  if (plan.BN == 16) return split_launch<T, false, false, 16>(p, e, plan.S, st);
+  if (plan.BN == 32) return split_launch<T, false, false, 32>(p, e, plan.S, st);
+  if (plan.BN == 64) return split_launch<T, false, false, 64>(p, e, plan.S, st);
+  return split_launch<T, false, false, 128>(p, e, plan.S, st);
 }
 template int product_sm100<__half>(const Product&, int, cudaStream_t);
 template int product_sm100<__nv_bfloat16>(const Product&, int, cudaStream_t);

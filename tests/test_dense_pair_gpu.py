@@ -1,7 +1,7 @@
 """Both tensor-core kernels of the dense layer on every shape of its tests: the
-CTA-pair kernel (256 x 256 tiles over two SMs) forced from one tile on, and the
-split kernel forced for all (CTB_DENSE_PAIR_TILES, read once per process, hence
-the subprocesses)."""
+CTA-pair kernel (256 x 256 tiles over two SMs) forced for all, and the split
+kernel forced for all (CTB_DENSE_PAIR, read once per process, hence the
+subprocesses)."""
 import os
 import subprocess
 import sys
@@ -13,9 +13,9 @@ pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-@pytest.mark.parametrize("tiles", ["1", "1000000000"])
-def test_forced_kernel(tiles):
-    env = dict(os.environ, CTB_DENSE_PAIR_TILES=tiles)
+@pytest.mark.parametrize("pair", ["1", "0"])
+def test_forced_kernel(pair):
+    env = dict(os.environ, CTB_DENSE_PAIR=pair)
     r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu",
                         os.path.join("tests", "test_dense_gpu.py")], cwd=ROOT, env=env,
                        capture_output=True, text=True, timeout=600)
