@@ -49,15 +49,11 @@ __device__ __forceinline__ void activate8(float (&z)[8]) {
   for (int i = 0; i < 8; i += 2) activate2<ACT>(z[i], z[i + 1]);
 }
 template <typename T>
-__device__ __forceinline__ void finish8(const Epilogue& e, int64_t r, int c, float (&z)[8]) {
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t r, int c, float (&z)[8],
+                                        const float (&bias)[8]) {
   const int n = min(8, e.cols - c);
-  if (e.bias) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n)
-        z[i] += e.bias_f32 ? static_cast<const float*>(e.bias)[c + i]
-                           : to_f32(static_cast<const T*>(e.bias)[c + i]);
-  }
+  for (int i = 0; i < 8; ++i) z[i] += bias[i];
   const bool whole = e.vec && n == 8;
   if (e.Z) {
     T* zp = static_cast<T*>(e.Z) + r * e.ldz + c;
@@ -251,6 +247,15 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
     }
     mma_commit_elect(done);
   }
+  // A thread's columns are the same for all its rows: 16 runs of 8 in a row, and
+  // the threads of the cluster a multiple of 16.
+  const int c = (int)(threadIdx.x % (SP_COLS / 8)) * 8;
+  float bias[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    bias[i] = !a.e.bias || c0 + c + i >= a.e.cols ? 0.f
+              : a.e.bias_f32 ? static_cast<const float*>(a.e.bias)[c0 + c + i]
+                             : to_f32(static_cast<const T*>(a.e.bias)[c0 + c + i]);
   // All roles meet at the finished accumulator. It exists on the way out of a
   // wait that gave up too; the host is told by the error word.
   mbar_wait_bounded(done, 0, abort_flag, ERR_BIT);
@@ -284,14 +289,20 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
 
   const uint32_t mine = smem_u32(partial);
   const int live_rows = (int)min((int64_t)BN, a.e.rows - r0);
-  for (int i = (int)rank * SP_THREADS + threadIdx.x; i < live_rows * (SP_COLS / 8);
-       i += (int)S * SP_THREADS) {
-    const int r = i / (SP_COLS / 8), c = i % (SP_COLS / 8) * 8;
-    if (c0 + c >= a.e.cols) continue;
+  for (int r = (int)(rank * SP_THREADS + threadIdx.x) / (SP_COLS / 8);
+       r < live_rows && c0 + c < a.e.cols; r += (int)S * (SP_THREADS / (SP_COLS / 8))) {
     float z[8] = {};
     for (uint32_t s = 0; s < S; ++s) {
-      const uint32_t from = mapa_shared(mine, s) + (uint32_t)(r * SP_COLS + c) * 4;
-      const float4 lo = ld_cluster_f4(from), hi = ld_cluster_f4(from + 16);
+      float4 lo, hi;
+      if (s == rank) {
+        const float4* from = reinterpret_cast<const float4*>(partial + r * SP_COLS + c);
+        lo = from[0];
+        hi = from[1];
+      } else {
+        const uint32_t from = mapa_shared(mine, s) + (uint32_t)(r * SP_COLS + c) * 4;
+        lo = ld_cluster_f4(from);
+        hi = ld_cluster_f4(from + 16);
+      }
       z[0] += lo.x;
       z[1] += lo.y;
       z[2] += lo.z;
@@ -301,7 +312,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
       z[6] += hi.z;
       z[7] += hi.w;
     }
-    finish8<T>(a.e, r0 + r, c0 + c, z);
+    finish8<T>(a.e, r0 + r, c0 + c, z, bias);
   }
   if (S > 1) cluster_sync_all();  // no CTA leaves while a peer may read its partials
 }
@@ -753,30 +764,32 @@ static bool rows16(const void* p, int64_t ld, int rows) {
 }
 
 // ---- which kernel, tile and split ------------------------------------------------------
-// A model of the two kernels' times in microseconds, fitted to 50 products of 1
-// to 512 rows and 512 to 14336 columns and k (on average 3% off the best tile and
-// split measured). A split CTA takes its k-blocks at 60 GB/s when alone on its SM,
-// two together at 100; 256 CTAs of clusters are sure to be resident at once, 296
-// single ones. A pair takes 0.31 us a k-block.
+// A model of the two kernels' times in microseconds, fitted to 965 runs: 91
+// products of 1 to 1536 rows, 640 to 14336 columns and 512 to 14336 k, each with
+// every tile and split (8% off a time; the choice by it takes 1.9% longer than
+// the best one measured, 14% at worst). A split CTA takes its k-blocks at 80 GB/s
+// when alone on its SM, two together at 150; 256 CTAs in clusters are sure to be
+// resident at once. A pair takes 0.3 us a k-block and 3 us a tile.
 struct Plan {
   int BN, S;  // BN = 0: the pair kernel
 };
 
-static double split_us(const Product& p, int BN, int S, int sms, double hbm_us) {
+static double split_us(const Product& p, int BN, int S, int sms, double moved) {
   const int64_t tiles = (int64_t)((p.cols + SP_COLS - 1) / SP_COLS) * ((p.rows + BN - 1) / BN);
   const int64_t ctas = tiles * S;
   const int kb = (p.depth + BK - 1) / BK, per = (kb + S - 1) / S;
   const double waves = (double)((ctas + 2 * sms - 1) / (2 * sms));
   const double both = ctas > sms ? 2 : 1;
   const double bytes = (double)per * sp_stage_bytes(BN);
-  const double load = waves * std::max(bytes / 60e3, both * bytes / 100e3);
-  return 4 + std::max(load, hbm_us) + waves * both * BN * 0.03 + (S > 1 ? 0.5 : 0) + 0.2 * S;
+  const double load = waves * std::max(bytes / 80e3, both * bytes / 150e3);
+  return 2.7 + std::max(load, moved / 6.4e6) + waves * both * BN * 0.03 + (S > 1 ? 0.7 : 0) +
+         0.28 * S;
 }
-static double pair_us(const Product& p, int pairs, double hbm_us) {
+static double pair_us(const Product& p, int pairs, double moved) {
   const int64_t tiles = (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
   const int kb = (p.depth + BK - 1) / BK;
   const double waves = (double)((tiles + pairs - 1) / pairs);
-  return 5.5 + std::max(waves * (1 + 0.31 * kb), hbm_us);
+  return 4 + std::max(waves * (3 + 0.3 * kb), moved / 4.7e6);
 }
 
 // CTB_DENSE_PAIR=0 never takes the pair kernel, =1 whenever a pair can be resident.
@@ -790,10 +803,10 @@ static int pair_mode() {
 
 static Plan choose_plan(const Product& p, int sms, int pairs) {
   const double out = 1 + (p.Z ? 1 : 0) + (p.R ? 1 : 0);
-  const double hbm_us = ((double)p.cols * p.depth + (double)p.rows * p.depth +
-                         out * (double)p.rows * p.cols) * 2 / 6e6;
+  const double moved = 2 * ((double)p.cols * p.depth + (double)p.rows * p.depth +
+                            out * (double)p.rows * p.cols);
   Plan best = {0, 1};
-  double us = pairs > 0 ? pair_us(p, pairs, hbm_us) : 1e30;
+  double us = pairs > 0 ? pair_us(p, pairs, moved) : 1e30;
   const int mode = pair_mode();
   if (mode == 1 && pairs > 0) return best;
   if (mode == 0) us = 1e30;
@@ -805,7 +818,7 @@ static Plan choose_plan(const Product& p, int sms, int pairs) {
     for (int S = 1; S <= 8; ++S) {
       if (S > 1 && (S > kb / 2 || tiles_c * tiles_r * S > 256)) break;
       if (S == 5 || S == 7) continue;
-      const double t = split_us(p, BN, S, sms, hbm_us);
+      const double t = split_us(p, BN, S, sms, moved);
       if (t < us) {
         us = t;
         best = {BN, S};
