@@ -303,6 +303,7 @@ __device__ __forceinline__ void choose(K (&key)[NV], Chosen* row, uint64_t* cand
     uint32_t t = key[0], bound = 0;
 #pragma unroll
     for (int v = 1; v < NV; ++v) t = max(t, key[v]);
+#pragma unroll 4
     for (int j = 0; j < rounds; ++j) {
       bound = __reduce_max_sync(FULL, t);
       if (t == bound) t = 0;
@@ -316,13 +317,19 @@ __device__ __forceinline__ void choose(K (&key)[NV], Chosen* row, uint64_t* cand
       total += __popc(b);
     }
     if (total <= 32) {
+      cand[lane] = 0;
+      __syncwarp();
 #pragma unroll
       for (int v = 0; v < NV; ++v)
         if (key[v] >= bound) cand[at[v]] = (uint64_t)key[v] << 32 | (uint32_t)~(lane * NV + v);
       __syncwarp();
-      const uint64_t mine = lane < total ? cand[lane] : 0;
+      const uint64_t mine = cand[lane];
       int place = 0;
-      for (int i = 0; i < total; ++i) place += cand[i] > mine;
+      for (int i = 0; i < total; i += 4) {  // zeros after the last are never above
+        const ulonglong2 p = *reinterpret_cast<const ulonglong2*>(cand + i);
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(cand + i + 2);
+        place += (p.x > mine) + (p.y > mine) + (q.x > mine) + (q.y > mine);
+      }
       if (lane >= total) place = lane;  // places that no expert is left for
       if (place < rounds) {
         row->id[place] = mine ? (int)~(uint32_t)mine : -1;
@@ -435,7 +442,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __res
   constexpr int ROWS = ROUTE_THREADS / LANES;
   constexpr int SLOTS = ROUTE_MAX_TOPK / LANES;  // places of a row per lane
   __shared__ Chosen sel_all[ROWS];
-  __shared__ uint64_t cand[LANES == 32 ? ROUTE_THREADS / 32 : 1][LANES == 32 ? 32 : 1];
+  __shared__ __align__(16) uint64_t cand[LANES == 32 ? ROUTE_THREADS / 32 : 1][LANES == 32 ? 32 : 1];
   __shared__ double scratch[GROUPED ? ROUTE_THREADS / 32 : 1]
                            [GROUPED ? ROUTE_MAX_EXPERTS + ROUTE_MAX_EXPERTS / 32 : 1];
   const int lane = threadIdx.x & 31, sub = lane % LANES, r = threadIdx.x / LANES;
@@ -499,6 +506,8 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __res
     xs[i] = id[i] >= 0 ? to_float(xr[id[i]]) : -INFINITY;
     m = fmaxf(m, xs[i]);
   }
+  // exp by ex2.approx: |x - shift| <= 24 gives 24 * 1.2e-7 relative error, 2e-7 at
+  // the differences of 1 to 2 that matter most.
   if (a.renorm) {
     // The common factor exp(-m) (sigmoid: exp(-min(m, 0))) leaves the shares as
     // they are and keeps them exact where all scores of a row underflow.
@@ -509,19 +518,21 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __res
     for (int i = 0; i < SLOTS; ++i) {
       w[i] = 0.f;
       if (id[i] >= 0) {
-        w[i] = a.sigmoid && xs[i] > 0.f ? 1.f : expf(xs[i] - shift);
-        if (a.sigmoid) w[i] /= 1.f + expf(-fabsf(xs[i]));
+        w[i] = a.sigmoid && xs[i] > 0.f ? 1.f : ex2_fast(kLog2e * (xs[i] - shift));
+        if (a.sigmoid) w[i] *= rcp_fast(1.f + ex2_fast(-kLog2e * fabsf(xs[i])));
       }
       sum += w[i];
     }
     sum = row_sum<LANES>(sum);
+    const float share = rcp_fast(sum);
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) w[i] = id[i] >= 0 ? w[i] / sum : 0.f;
+    for (int i = 0; i < SLOTS; ++i) w[i] = id[i] >= 0 ? w[i] * share : 0.f;
   } else {
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i)
       w[i] = id[i] < 0 ? 0.f
-                       : a.sigmoid ? 1.f / (1.f + expf(-xs[i])) : expf(xs[i] - top) / total;
+             : a.sigmoid ? rcp_fast(1.f + ex2_fast(-kLog2e * xs[i]))
+                         : ex2_fast(kLog2e * (xs[i] - top)) * scale_of;
   }
   if (in_range) {
 #pragma unroll
