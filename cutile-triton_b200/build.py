@@ -1,4 +1,6 @@
-"""Builds libcutile_b200.so in-tree from csrc/*.cu for sm_100a with nvcc.
+"""Builds libcutile_b200.so in-tree from csrc/*.cu for sm_100a with nvcc, and
+_torch_binding.so (the layer calls' Python binding) from csrc/torch_binding.cpp
+with g++.
 
 Usage: python cutile-triton_b200/build.py [--force]
 The library is rebuilt when any source or the public header is newer than it.
@@ -12,6 +14,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "cutile_b200", "libcutile_b200.so")
+BINDING = os.path.join(HERE, "cutile_b200", "_torch_binding.so")
 HEADER = os.path.join(ROOT, "include", "cutile_b200.h")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -34,6 +37,30 @@ def _needs(target, deps):
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def build_binding(force=False):
+    """Compiles csrc/torch_binding.cpp against the torch that this interpreter
+    imports. No run path is recorded: the libraries it names are the ones that
+    `import torch` has loaded by then."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    if not force and not _needs(BINDING, [src, HEADER, torch.__file__]):
+        return BINDING
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    inc = cpp_extension.include_paths() + [sysconfig.get_paths()["include"],
+                                           os.path.join(cuda, "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), src, "-o", BINDING]
+    cmd += [a for i in inc for a in ("-isystem", i)]
+    cmd += ["-L" + p for p in cpp_extension.library_paths()]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    subprocess.run(cmd, check=True)
+    return BINDING
 
 
 def build(force=False, verbose=False, defines=(), lib=None, obj=None):
@@ -64,3 +91,4 @@ def build(force=False, verbose=False, defines=(), lib=None, obj=None):
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_binding(force="--force" in sys.argv))

@@ -283,109 +283,42 @@ def moe_gemm(A, B, sorted_ids, expert_ids, ntp, topk, weights=None, out=None, wo
     return out
 
 
-# ---- argument checks of the layer calls below ------------------------------------
-def _need(ok, code, msg):
-    if not ok:
-        raise _lib.B200Error(code, msg)
+# ---- mixture-of-experts layer -----------------------------------------------------
+# These calls go through _torch_binding (csrc/torch_binding.cpp), which checks
+# the arguments, allocates the outputs and calls the C ABI on the current stream
+# of the tensors' device.
+_binding = None
+_BOUND = ("ctb_last_error", "ctb_dense_fwd_workspace_bytes", "ctb_dense_fwd",
+          "ctb_dense_bwd_workspace_bytes", "ctb_dense_bwd", "ctb_moe_route", "ctb_moe_route_bwd",
+          "ctb_moe_combine", "ctb_moe_combine_bwd")
 
 
-def _need_rows(t, what):
-    """A 2-D CUDA tensor with contiguous rows: what a call's first matrix must
-    be, whose shape, dtype and device the others are held to."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        raise _lib.B200Error(-1, f"{what}: expected CUDA tensors")
-    if t.dim() != 2:
-        raise _lib.B200Error(-3, f"{what}: expected a matrix, got {t.dim()} dimensions")
-    if t.stride(1) != 1 and t.shape[1] > 1:
-        raise _lib.B200Error(-4, f"{what}: rows must be contiguous")
+def _bind():
+    """Loads the binding and hands it the library's entry points; a missing
+    binding is an error (there is no fallback path)."""
+    global _binding
+    L = _lib.load()
+    try:
+        from . import _torch_binding
+    except ImportError as e:
+        raise _lib.B200Error(-8, f"_torch_binding.so cannot be loaded ({e}); build it with "
+                                 "`python cutile-triton_b200/build.py`") from e
+    _torch_binding.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BOUND},
+                        _lib.B200Error)
+    _binding = _torch_binding
+    return _binding
 
 
-def _need_matrix(t, rows, cols, dtype, device, what):
-    """A (rows, cols) CUDA matrix of `dtype` on `device` with contiguous rows."""
-    if not (isinstance(t, torch.Tensor) and t.device == device):
-        at = t.device if isinstance(t, torch.Tensor) else type(t).__name__
-        raise _lib.B200Error(-1, f"{what}: expected a CUDA tensor on {device}, got {at}")
-    if t.dtype != dtype:
-        raise _lib.B200Error(-2, f"{what}: expected {dtype}, got {t.dtype}")
-    if t.shape != (rows, cols):
-        raise _lib.B200Error(-3, f"{what}: expected shape ({rows}, {cols}), got {tuple(t.shape)}")
-    if t.stride(1) != 1 and cols > 1:
-        raise _lib.B200Error(-4, f"{what}: rows must be contiguous")
-
-
-def _need_packed(t, shape, dtype, device, what):
-    """A contiguous CUDA tensor of exactly this shape and dtype."""
-    if not (isinstance(t, torch.Tensor) and t.device == device):
-        at = t.device if isinstance(t, torch.Tensor) else type(t).__name__
-        raise _lib.B200Error(-1, f"{what}: expected a CUDA tensor on {device}, got {at}")
-    if t.dtype != dtype:
-        raise _lib.B200Error(-2, f"{what}: expected {dtype}, got {t.dtype}")
-    if t.shape != shape:
-        raise _lib.B200Error(-3, f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise _lib.B200Error(-4, f"{what}: must be contiguous")
-
-
-def _new_matrix(rows, cols, dtype, device):
-    # empty_strided takes 1.6 us, empty with a shape 2.4
-    return torch.empty_strided((rows, cols), (cols if cols > 0 else 1, 1), dtype=dtype, device=device)
-
-
-def _ld(t):
-    """Row stride for the C ABI. A single row has none that matters (torch
-    gives any number for it): its length does."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-# The current stream's handle without building a torch Stream object (3 us a call).
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _call_on(device, name, *args):
-    """One library call on the current stream of `device`, which need not be
-    the current device."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(device):
-            rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
-    if rc:
-        _lib.check(rc)
+def _code(table, key, what):
+    try:
+        return table[key]
+    except (KeyError, TypeError):
+        raise _lib.B200Error(-1, f"{what} {key!r}") from None
 
 
 # ---- dense layer ------------------------------------------------------------------
 _ACTS = {"none": _lib.CTB_ACT_NONE, "relu": _lib.CTB_ACT_RELU, "gelu": _lib.CTB_ACT_GELU,
          "gelu_tanh": _lib.CTB_ACT_GELU_TANH, "silu": _lib.CTB_ACT_SILU}
-
-
-def _dense_operands(k, A_t, B_t, act):
-    """Checks the weight (K, M) and the activations (N, K) -> (M, N, K, dtype, device)."""
-    _need_rows(A_t, k)
-    _need_rows(B_t, k)
-    if act not in _ACTS:
-        raise _lib.B200Error(-1, f"{k}: unknown activation {act!r}")
-    dt, dev = A_t.dtype, A_t.device
-    if (dt is not torch.float16 and dt is not torch.bfloat16) or B_t.dtype is not dt:
-        raise _lib.B200Error(-2, f"{k}: both float16 or both bfloat16, got {dt} and {B_t.dtype}")
-    K, M = A_t.shape
-    N, kb = B_t.shape
-    if kb != K:
-        raise _lib.B200Error(-3, f"{k}: A_t must be (K, M), B_t (N, K)")
-    if B_t.device != dev:
-        raise _lib.B200Error(-1, f"{k}: A_t is on {dev}, B_t on {B_t.device}")
-    return M, N, K, dt, dev
-
-
-def _workspace(nbytes, device):
-    """Scratch of one call: from torch's allocator, which keeps it to this
-    stream's order and, in a capture, to the graph."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
 def dense(A_t, B_t, bias=None, act="none", residual=None, out=None, preact=None):
@@ -396,29 +329,8 @@ def dense(A_t, B_t, bias=None, act="none", residual=None, out=None, preact=None)
     float32; `preact` (N, M), when given, receives the value before the
     activation, which :func:`dense_bwd` needs. `out` may be `residual`. Sums
     are float32; each output is rounded once."""
-    M, N, K, dt, dev = _dense_operands("dense", A_t, B_t, act)
-    if bias is not None:
-        _need_packed(bias, (M,), bias.dtype if bias.dtype == torch.float32 else dt, dev,
-                     "dense: bias")
-    if residual is not None:
-        _need_matrix(residual, N, M, dt, dev, "dense: residual")
-    if preact is not None:
-        _need_matrix(preact, N, M, dt, dev, "dense: preact")
-    if out is None:
-        out = _new_matrix(N, M, dt, dev)
-    else:
-        _need_matrix(out, N, M, dt, dev, "dense: out")
-    lda, ldb = _ld(A_t), _ld(B_t)
-    pa, pb = A_t.data_ptr(), B_t.data_ptr()
-    nws, ws = 0, None
-    if (pa | pb) & 15 or (lda | ldb) & 7:
-        nws = _lib.load().ctb_dense_fwd_workspace_bytes(pa, pb, M, N, K, lda, ldb)
-        ws = _workspace(nws, dev)
-    _call_on(dev, "ctb_dense_fwd", _DT[dt], pa, pb, _ptr(bias),
-             0 if bias is None else _DT[bias.dtype], _ptr(residual), _ptr(preact), out.data_ptr(),
-             M, N, K, lda, ldb, 0 if residual is None else _ld(residual),
-             0 if preact is None else _ld(preact), _ld(out), _ACTS[act], _ptr(ws), nws)
-    return out
+    return (_binding or _bind()).dense(A_t, B_t, bias, _code(_ACTS, act, "dense: unknown activation"),
+                                       residual, out, preact)
 
 
 def dense_bwd(dC_t, A_t, B_t, act="none", preact=None, dA_t=None, dB_t=None, dbias=None,
@@ -426,44 +338,12 @@ def dense_bwd(dC_t, A_t, B_t, act="none", preact=None, dA_t=None, dB_t=None, dbi
     """Gradients of :func:`dense` from dC_t (N, M) -> (dA_t (K, M), dB_t (N, K),
     dbias (M) float32), None for those not needed. `preact` is the forward
     call's (not used without an activation). The residual's gradient is dC_t."""
-    M, N, K, dt, dev = _dense_operands("dense_bwd", A_t, B_t, act)
-    _need_matrix(dC_t, N, M, dt, dev, "dense_bwd: dC_t")
-    if act != "none":
-        _need(preact is not None, -1, "dense_bwd: an activation's gradient needs preact")
-        _need_matrix(preact, N, M, dt, dev, "dense_bwd: preact")
-    else:
-        preact = None
-    if not need_dA:
-        dA_t = None
-    elif dA_t is None:
-        dA_t = _new_matrix(K, M, dt, dev)
-    else:
-        _need_matrix(dA_t, K, M, dt, dev, "dense_bwd: dA_t")
-    if not need_dB:
-        dB_t = None
-    elif dB_t is None:
-        dB_t = _new_matrix(N, K, dt, dev)
-    else:
-        _need_matrix(dB_t, N, K, dt, dev, "dense_bwd: dB_t")
-    if not need_dbias:
-        dbias = None
-    elif dbias is None:
-        dbias = torch.empty(M, dtype=torch.float32, device=dev)
-    else:
-        _need_packed(dbias, (M,), torch.float32, dev, "dense_bwd: dbias")
-    lddc, lda, ldb = _ld(dC_t), _ld(A_t), _ld(B_t)
-    pd, pa, pb = dC_t.data_ptr(), A_t.data_ptr(), B_t.data_ptr()
-    nws = _lib.load().ctb_dense_bwd_workspace_bytes(pd, pa, pb, M, N, K, lddc, lda, ldb, _ACTS[act],
-                                                    1 if need_dbias else 0)
-    ws = _workspace(nws, dev)
-    _call_on(dev, "ctb_dense_bwd", _DT[dt], pd, pa, pb, _ptr(preact), _ptr(dA_t), _ptr(dB_t),
-             _ptr(dbias), M, N, K, lddc, lda, ldb, 0 if preact is None else _ld(preact),
-             0 if dA_t is None else _ld(dA_t), 0 if dB_t is None else _ld(dB_t), _ACTS[act],
-             _ptr(ws), nws)
-    return dA_t, dB_t, dbias
+    return (_binding or _bind()).dense_bwd(
+        dC_t, A_t, B_t, _code(_ACTS, act, "dense_bwd: unknown activation"), preact, dA_t, dB_t,
+        dbias, need_dA, need_dB, need_dbias)
 
 
-# ---- mixture-of-experts layer: routing and combine ------------------------------
+# ---- routing and combine ---------------------------------------------------------------
 _SCORES = {"softmax": _lib.CTB_SCORE_SOFTMAX, "sigmoid": _lib.CTB_SCORE_SIGMOID}
 
 
@@ -481,61 +361,18 @@ def moe_route(logits, topk, score="softmax", bias=None, groups=1, topk_groups=No
     the sum of the chosen s. An expert with a logit or c of -inf or NaN is not
     available; places no expert is left for get id -1 and weight 0 (a row of
     -inf, a padding token, goes to no expert). E <= 256, topk <= 32."""
-    _need_rows(logits, "moe_route: logits")
-    _need(isinstance(topk, int) and topk >= 1, -3, "moe_route: topk must be positive")
-    if score not in _SCORES:
-        raise _lib.B200Error(-1, f"moe_route: unknown score {score!r}")
-    T, E = logits.shape
-    dev = logits.device
-    if bias is not None:
-        _need_packed(bias, (E,), torch.float32, dev, "moe_route: bias")
-    if weights is None:
-        weights = _new_matrix(T, topk, torch.float32, dev)
-    else:
-        _need_packed(weights, (T, topk), torch.float32, dev, "moe_route: weights")
-    if ids is None:
-        ids = _new_matrix(T, topk, torch.int32, dev)
-    else:
-        _need_packed(ids, (T, topk), torch.int32, dev, "moe_route: ids")
-    _call_on(dev, "ctb_moe_route", _DT.get(logits.dtype, 0), logits.data_ptr(), _ptr(bias),
-             weights.data_ptr(), ids.data_ptr(), T, E, topk, _ld(logits), _SCORES[score], groups,
-             groups if topk_groups is None else topk_groups, group_top, 1 if renorm else 0, scale)
-    return weights, ids
+    return (_binding or _bind()).moe_route(
+        logits, topk, _code(_SCORES, score, "moe_route: unknown score"), bias, groups, topk_groups,
+        group_top, renorm, scale, weights, ids)
 
 
 def moe_route_bwd(dweights, logits, ids, score="softmax", renorm=True, scale=1.0, dlogits=None):
     """Gradient of :func:`moe_route`'s weights: dlogits (T, E, dtype of the
     logits) from dweights (T, topk) and the ids of the forward call. The
     choice and its bias have no gradient."""
-    _need_rows(logits, "moe_route_bwd: logits")
-    _need_rows(ids, "moe_route_bwd: ids")
-    if score not in _SCORES:
-        raise _lib.B200Error(-1, f"moe_route_bwd: unknown score {score!r}")
-    T, E = logits.shape
-    topk = ids.shape[1]
-    dev = logits.device
-    _need_packed(ids, (T, topk), torch.int32, dev, "moe_route_bwd: ids")
-    _need_packed(dweights, (T, topk), torch.float32, dev, "moe_route_bwd: dweights")
-    if dlogits is None:
-        dlogits = _new_matrix(T, E, logits.dtype, dev)
-    else:
-        _need_matrix(dlogits, T, E, logits.dtype, dev, "moe_route_bwd: dlogits")
-    _call_on(dev, "ctb_moe_route_bwd", _DT.get(logits.dtype, 0), dweights.data_ptr(), logits.data_ptr(),
-             ids.data_ptr(), dlogits.data_ptr(), T, E, topk, _ld(logits), _ld(dlogits),
-             _SCORES[score], 1 if renorm else 0, scale)
-    return dlogits
-
-
-def _combine_args(k, rows, topk, weights, ids, num_experts, dev):
-    if not (isinstance(topk, int) and topk >= 1 and rows % topk == 0):
-        raise _lib.B200Error(-3, f"{k}: y must have T * topk rows")
-    T = rows // topk
-    if weights is not None:
-        _need_packed(weights, (T, topk), torch.float32, dev, "weights")
-    if ids is not None:
-        _need_packed(ids, (T, topk), torch.int32, dev, "ids")
-        _need(num_experts is not None, -1, "ids need num_experts")
-    return T, int(num_experts) if ids is not None else 0
+    return (_binding or _bind()).moe_route_bwd(
+        dweights, logits, ids, _code(_SCORES, score, "moe_route_bwd: unknown score"), renorm, scale,
+        dlogits)
 
 
 def moe_combine(y, topk, weights=None, ids=None, num_experts=None, residual=None, out=None):
@@ -546,20 +383,7 @@ def moe_combine(y, topk, weights=None, ids=None, num_experts=None, residual=None
     `ids` (T, topk) int32 and `num_experts`, slots with an id outside
     [0, num_experts) are skipped: no expert wrote their rows, which are not
     read. `out` may be `residual`."""
-    _need_rows(y, "moe_combine: y")
-    rows, N = y.shape
-    dev = y.device
-    T, E = _combine_args("moe_combine", rows, topk, weights, ids, num_experts, dev)
-    if residual is not None:
-        _need_matrix(residual, T, N, y.dtype, dev, "moe_combine: residual")
-    if out is None:
-        out = _new_matrix(T, N, y.dtype, dev)
-    else:
-        _need_matrix(out, T, N, y.dtype, dev, "moe_combine: out")
-    _call_on(dev, "ctb_moe_combine", _DT.get(y.dtype, 0), y.data_ptr(), _ptr(weights), _ptr(ids),
-             _ptr(residual), out.data_ptr(), T, topk, N, E, _ld(y),
-             0 if residual is None else _ld(residual), _ld(out))
-    return out
+    return (_binding or _bind()).moe_combine(y, topk, weights, ids, num_experts, residual, out)
 
 
 def moe_combine_bwd(dout, y, topk, weights=None, ids=None, num_experts=None, dy=None,
@@ -567,29 +391,8 @@ def moe_combine_bwd(dout, y, topk, weights=None, ids=None, num_experts=None, dy=
     """Gradients of :func:`moe_combine` -> (dy (T * topk, N), dweights (T, topk)
     float32, None without weights). Skipped slots get zeros. The gradient of
     the residual is `dout`. Without weights `y` is not used and may be None."""
-    _need_rows(dout, "moe_combine_bwd: dout")
-    T, N = dout.shape
-    dev = dout.device
-    _need(isinstance(topk, int) and topk >= 1, -3, "moe_combine_bwd: topk must be positive")
-    rows = T * topk
-    T, E = _combine_args("moe_combine_bwd", rows, topk, weights, ids, num_experts, dev)
-    if weights is None:
-        _need(dweights is None, -1, "moe_combine_bwd: dweights without weights")
-        y = None
-    else:
-        _need_matrix(y, rows, N, dout.dtype, dev, "moe_combine_bwd: y")
-        if dweights is None:
-            dweights = _new_matrix(T, topk, torch.float32, dev)
-        else:
-            _need_packed(dweights, (T, topk), torch.float32, dev, "moe_combine_bwd: dweights")
-    if dy is None:
-        dy = _new_matrix(rows, N, dout.dtype, dev)
-    else:
-        _need_matrix(dy, rows, N, dout.dtype, dev, "moe_combine_bwd: dy")
-    _call_on(dev, "ctb_moe_combine_bwd", _DT.get(dout.dtype, 0), dout.data_ptr(), _ptr(y), _ptr(weights),
-             _ptr(ids), dy.data_ptr(), _ptr(dweights), T, topk, N, E, _ld(dout),
-             0 if y is None else _ld(y), _ld(dy))
-    return dy, dweights
+    return (_binding or _bind()).moe_combine_bwd(dout, y, topk, weights, ids, num_experts, dy,
+                                                 dweights)
 
 
 # ---- host-buffer calls (three-stream chunk pipeline inside the library) -------
