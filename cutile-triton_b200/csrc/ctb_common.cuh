@@ -66,6 +66,46 @@ __device__ __forceinline__ void flag_device_error(unsigned int bit) {
   atomicOr(&g_device_error, bit);
 }
 
+// ---- programmatic dependent launch ---------------------------------------------
+// A kernel launched with launch_overlapped may start while its predecessor on
+// the stream still runs, once every CTA of that one has called
+// let_next_start() (or ended); it touches global memory only after
+// wait_for_previous(), which returns when the predecessor has completed and its
+// writes are visible. That hides a launch's latency and a kernel's set-up behind
+// the predecessor's tail. A kernel that allocates tensor memory lets the next
+// start only after the allocation: CTAs of the next one hold theirs while they
+// wait.
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... P, typename... A>
+inline int launch_overlapped(const char* what, void (*kernel)(P...), dim3 grid, int threads,
+                             int smem, int cluster, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_fail(e, what);
+  }
+  return CTB_OK;
+}
+
 // ---- vector memory helpers --------------------------------------------------
 // Streaming loads: data is read once, do not allocate in L1.
 __device__ __forceinline__ float4 ld_stream_f4(const float* p) {

@@ -22,6 +22,8 @@ namespace {
 // ---- a product over nothing: act(bias) + R ---------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) product_empty_kernel(const Product p) {
+  let_next_start();
+  wait_for_previous();
   const int64_t total = (int64_t)p.rows * p.cols;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * 256) {
@@ -53,6 +55,8 @@ int64_t packed_bytes(int64_t lines, int64_t len) { return round256(2 * lines * r
 __global__ void __launch_bounds__(256)
     pack_kernel(const uint16_t* __restrict__ src, uint4* __restrict__ dst, int64_t lines, int len,
                 int64_t ld) {
+  let_next_start();
+  wait_for_previous();
   const int runs = (len + 7) / 8;
   const int64_t total = lines * runs;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
@@ -75,20 +79,21 @@ int pack_operand(const void** p, int64_t* ld, int64_t lines, int64_t len, uint8_
                  cudaStream_t st) {
   if (lines == 0 || len == 0 || tma_lines(*p, *ld, lines)) return CTB_OK;
   const int64_t grid = std::min<int64_t>((lines * ((len + 7) / 8) + 255) / 256, 16ll * sms);
-  pack_kernel<<<(unsigned)grid, 256, 0, st>>>(static_cast<const uint16_t*>(*p),
-                                              reinterpret_cast<uint4*>(*ws), lines, (int)len, *ld);
+  const int rc = launch_overlapped("pack_kernel", pack_kernel, dim3((unsigned)grid), 256, 0, 0, st,
+                                   static_cast<const uint16_t*>(*p), reinterpret_cast<uint4*>(*ws),
+                                   lines, (int)len, *ld);
   *p = *ws;
   *ld = round8(len);
   *ws += packed_bytes(lines, len);
-  return launch_status("pack_kernel");
+  return rc;
 }
 
 template <typename T>
 int product(const Product& p, int sms, cudaStream_t st) {
   if (p.depth > 0) return product_sm100<T>(p, sms, st);
   const int64_t grid = std::min<int64_t>(((int64_t)p.rows * p.cols + 255) / 256, 16ll * sms);
-  product_empty_kernel<T><<<(unsigned)grid, 256, 0, st>>>(p);
-  return launch_status("product_empty_kernel");
+  return launch_overlapped("product_empty_kernel", product_empty_kernel<T>, dim3((unsigned)grid),
+                           256, 0, 0, st, p);
 }
 
 // ---- dZ = dC .* act'(Z) and its column sums ---------------------------------------------
@@ -124,6 +129,8 @@ __global__ void __launch_bounds__(SLOPE_THREADS, 4)
     slope_kernel(const T* __restrict__ dC, const T* __restrict__ Z, T* __restrict__ dZ,
                  float* __restrict__ partial, int N, int M, int64_t lddc, int64_t ldz,
                  int64_t lddz, int span) {
+  let_next_start();
+  wait_for_previous();
   __shared__ float red[SLOPE_WARPS][32 * W];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int c = (int)(blockIdx.x * 32 + lane) * W;
@@ -183,6 +190,8 @@ __global__ void __launch_bounds__(SLOPE_THREADS, 4)
 // Sums the spans: 32 columns a CTA, eight threads a column, joined in order.
 __global__ void __launch_bounds__(256)
     fold_kernel(const float* __restrict__ partial, float* __restrict__ out, int M, int spans) {
+  let_next_start();
+  wait_for_previous();
   __shared__ float red[8][32];
   const int cl = threadIdx.x % 32, g = threadIdx.x / 32, c = blockIdx.x * 32 + cl;
   float s = 0.f;
@@ -216,8 +225,8 @@ int slope_launch(const T* dC, const T* Z, T* dZ, float* sums, int N, int M, int6
     case CTB_ACT_SILU: k = slope_kernel<T, W, CTB_ACT_SILU>; break;
     default: break;
   }
-  k<<<grid, SLOPE_THREADS, 0, st>>>(dC, Z, dZ, sums, N, M, lddc, ldz, lddz, (N + spans - 1) / spans);
-  return launch_status("slope_kernel");
+  return launch_overlapped("slope_kernel", k, grid, SLOPE_THREADS, 0, 0, st, dC, Z, dZ, sums, N, M,
+                           lddc, ldz, lddz, (N + spans - 1) / spans);
 }
 
 // dZ goes to the workspace where it is not dC itself: with an activation, or
@@ -252,8 +261,9 @@ int dense_bwd(const T* dC, const T* A, const T* B, const T* Z, T* dA, T* dB, flo
                   : slope_launch<T, 1>(dC, Z, dz, sums, N, M, lddc, ldz, lddz, act, spans, st);
     if (rc) return rc;
     if (dbias && spans > 1) {
-      fold_kernel<<<(M + 31) / 32, 256, 0, st>>>(sums, dbias, M, spans);
-      if ((rc = launch_status("fold_kernel"))) return rc;
+      rc = launch_overlapped("fold_kernel", fold_kernel, dim3((M + 31) / 32), 256, 0, 0, st, sums,
+                             dbias, M, spans);
+      if (rc) return rc;
     }
   }
   if (dB && N > 0 && K > 0) {

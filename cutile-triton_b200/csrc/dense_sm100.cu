@@ -189,6 +189,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  let_next_start();
+  wait_for_previous();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -415,6 +417,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   cluster_sync_all();  // barriers initialised in both CTAs before any cross-CTA use
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  let_next_start();
+  wait_for_previous();
   const uint32_t full_leader = mapa_shared(smem_u32(&full[0]), 0);
 
   if (warp == 0) {
@@ -684,21 +688,6 @@ int pair_attrs() {
   if (!rc) rc = pair_attr<T, true, true>();
   return rc;
 }
-static void cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, dim3 grid,
-                           int threads, int smem, int cluster, cudaStream_t st) {
-  *cfg = {};
-  attr->id = cudaLaunchAttributeClusterDimension;
-  attr->val.clusterDim.x = cluster;
-  attr->val.clusterDim.y = 1;
-  attr->val.clusterDim.z = 1;
-  cfg->gridDim = grid;
-  cfg->blockDim = dim3(threads, 1, 1);
-  cfg->dynamicSmemBytes = smem;
-  cfg->stream = st;
-  cfg->attrs = attr;
-  cfg->numAttrs = 1;
-}
-
 template <typename T, bool Q_MN, bool P_MN, int BN>
 int split_attr() {
   CTB_CUDA_CHECK(cudaFuncSetAttribute(product_split_kernel<T, Q_MN, P_MN, BN>,
@@ -735,9 +724,17 @@ int device_setup(int* pairs_out) {
   if (int rc = split_attrs<__nv_bfloat16>()) return rc;
   if (int rc = pair_attrs<__half>()) return rc;
   if (int rc = pair_attrs<__nv_bfloat16>()) return rc;
-  cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr;
-  cluster_config(&cfg, &attr, dim3(2), PR_THREADS, PR_SMEM, 2, nullptr);
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2);
+  cfg.blockDim = dim3(PR_THREADS);
+  cfg.dynamicSmemBytes = PR_SMEM;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
   int pairs = 0;
   CTB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&pairs, product_pair_kernel<__half, false, true>, &cfg));
   if (dev < 64) {
@@ -839,12 +836,9 @@ int split_launch(const Product& p, const Epilogue& e, int S, cudaStream_t st) {
   a.num_kb = (p.depth + BK - 1) / BK;
   const int64_t tiles_c = (p.cols + SP_COLS - 1) / SP_COLS, tiles_r = ((int64_t)p.rows + BN - 1) / BN;
   if (tiles_r > 65535) return set_error(CTB_ERR_SHAPE, "dense: too many rows");
-  cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr;
-  cluster_config(&cfg, &attr, dim3((unsigned)(tiles_c * S), (unsigned)tiles_r, 1), SP_THREADS,
-                 sp_smem(BN), S, st);
-  CTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, product_split_kernel<T, Q_MN, P_MN, BN>, tmQ, tmP, a));
-  return launch_status("product_split_kernel");
+  return launch_overlapped("product_split_kernel", product_split_kernel<T, Q_MN, P_MN, BN>,
+                           dim3((unsigned)(tiles_c * S), (unsigned)tiles_r), SP_THREADS,
+                           sp_smem(BN), S, st, tmQ, tmP, a);
 }
 
 // A 16-bit matrix as boxes of 32 rows x 32 columns for the epilogue; a matrix
@@ -878,13 +872,9 @@ int pair_launch(const Product& p, const Epilogue& e, int pairs, cudaStream_t st)
   a.tiles_r = (p.rows + 255) / 256;
   a.tiles_c = (p.cols + 255) / 256;
   a.num_tiles = (int64_t)a.tiles_r * a.tiles_c;
-  cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr;
-  cluster_config(&cfg, &attr, dim3((unsigned)(2 * std::min<int64_t>(a.num_tiles, pairs))),
-                 PR_THREADS, PR_SMEM, 2, st);
-  CTB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, product_pair_kernel<T, P_MN, Q_MN>, tmP, tmQ, tmD, tmZ,
-                                    tmR, a));
-  return launch_status("product_pair_kernel");
+  return launch_overlapped("product_pair_kernel", product_pair_kernel<T, P_MN, Q_MN>,
+                           dim3((unsigned)(2 * std::min<int64_t>(a.num_tiles, pairs))), PR_THREADS,
+                           PR_SMEM, 2, st, tmP, tmQ, tmD, tmZ, tmR, a);
 }
 
 // The product on the tensor cores. Operands start on 16-byte boundaries, their

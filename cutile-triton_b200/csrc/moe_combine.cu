@@ -94,6 +94,8 @@ struct CombineArgs {
 // TOPK > 0: that many slots, all loads in flight; 0: any number, in turn.
 template <typename T, int W, int TOPK>
 __global__ void __launch_bounds__(COMBINE_THREADS) moe_combine_kernel(const CombineArgs<T> a) {
+  let_next_start();
+  wait_for_previous();
   const int64_t i = (int64_t)blockIdx.x * COMBINE_THREADS + threadIdx.x;
   if (i >= a.items) return;
   const int64_t t = a.items >> 31 ? i / a.runs : (int64_t)((uint32_t)i / (uint32_t)a.runs);
@@ -162,6 +164,8 @@ struct CombineBwdArgs {
 template <typename T, int W>
 __global__ void __launch_bounds__(COMBINE_THREADS)
     moe_combine_bwd_kernel(const CombineBwdArgs<T> a) {
+  let_next_start();
+  wait_for_previous();
   const int lane = threadIdx.x & 31;
   const int64_t s = (int64_t)blockIdx.x * (COMBINE_THREADS / 32) + threadIdx.x / 32;
   if (s >= a.slots) return;
@@ -235,8 +239,8 @@ int combine_launch(const CombineArgs<T>& a, cudaStream_t st) {
     case 8: k = moe_combine_kernel<T, W, 8>; break;
     default: break;
   }
-  k<<<(unsigned)grid, COMBINE_THREADS, 0, st>>>(a);
-  return launch_status("moe_combine_kernel");
+  return launch_overlapped("moe_combine_kernel", k, dim3((unsigned)grid), COMBINE_THREADS, 0, 0, st,
+                           a);
 }
 
 template <typename T>
@@ -255,9 +259,9 @@ int combine_bwd_dispatch(const CombineBwdArgs<T>& a, cudaStream_t st) {
   if (grid > 0x7fffffff) return set_error(CTB_ERR_SHAPE, "moe_combine_bwd: too many slots");
   const bool vec = a.N % 8 == 0 && rows16(a.dout, a.lddo) && rows16(a.dy, a.lddy) &&
                    (!a.weights || rows16(a.y, a.ldy));
-  if (vec) moe_combine_bwd_kernel<T, 8><<<(unsigned)grid, COMBINE_THREADS, 0, st>>>(a);
-  else moe_combine_bwd_kernel<T, 1><<<(unsigned)grid, COMBINE_THREADS, 0, st>>>(a);
-  return launch_status("moe_combine_bwd_kernel");
+  return launch_overlapped("moe_combine_bwd_kernel",
+                           vec ? moe_combine_bwd_kernel<T, 8> : moe_combine_bwd_kernel<T, 1>,
+                           dim3((unsigned)grid), COMBINE_THREADS, 0, 0, st, a);
 }
 
 int combine_check(const std::string& n, int dtype, int T, int topk, int N, int E, bool ids) {

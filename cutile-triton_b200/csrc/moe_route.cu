@@ -445,6 +445,8 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __res
   __shared__ __align__(16) uint64_t cand[LANES == 32 ? ROUTE_THREADS / 32 : 1][LANES == 32 ? 32 : 1];
   __shared__ double scratch[GROUPED ? ROUTE_THREADS / 32 : 1]
                            [GROUPED ? ROUTE_MAX_EXPERTS + ROUTE_MAX_EXPERTS / 32 : 1];
+  let_next_start();
+  wait_for_previous();
   const int lane = threadIdx.x & 31, sub = lane % LANES, r = threadIdx.x / LANES;
   const int64_t t = (int64_t)blockIdx.x * ROWS + r;
   const bool in_range = t < a.T;
@@ -571,6 +573,8 @@ __global__ void __launch_bounds__(ROUTE_THREADS)
   constexpr int ROWS = ROUTE_THREADS / LANES;
   constexpr int SLOTS = ROUTE_MAX_TOPK / LANES;
   __shared__ int2 slot_all[ROWS][ROUTE_MAX_TOPK];  // (expert, gradient bits) of each place
+  let_next_start();
+  wait_for_previous();
   const int lane = threadIdx.x & 31, sub = lane % LANES, r = threadIdx.x / LANES;
   const int64_t t = (int64_t)blockIdx.x * ROWS + r;
   const bool in_range = t < a.T;
@@ -688,11 +692,9 @@ template <typename T, int LANES, int NV, bool GROUPED>
 int route_launch(const T* x, const RouteArgs& a, cudaStream_t st) {
   const int rows = ROUTE_THREADS / LANES;
   const unsigned grid = (unsigned)(((int64_t)a.T + rows - 1) / rows);
-  if (runs_ok<T>(x, a.ldx, a.E, NV))
-    moe_route_kernel<T, LANES, NV, true, GROUPED><<<grid, ROUTE_THREADS, 0, st>>>(x, a);
-  else
-    moe_route_kernel<T, LANES, NV, false, GROUPED><<<grid, ROUTE_THREADS, 0, st>>>(x, a);
-  return launch_status("moe_route_kernel");
+  auto k = runs_ok<T>(x, a.ldx, a.E, NV) ? moe_route_kernel<T, LANES, NV, true, GROUPED>
+                                         : moe_route_kernel<T, LANES, NV, false, GROUPED>;
+  return launch_overlapped("moe_route_kernel", k, dim3(grid), ROUTE_THREADS, 0, 0, st, x, a);
 }
 template <typename T>
 int route_dispatch(const T* x, const RouteArgs& a, cudaStream_t st) {
@@ -714,11 +716,11 @@ template <typename T, int LANES, int NV>
 int route_bwd_launch(const T* x, T* dx, const RouteBwdArgs& a, cudaStream_t st) {
   const int rows = ROUTE_THREADS / LANES;
   const unsigned grid = (unsigned)(((int64_t)a.T + rows - 1) / rows);
-  if (runs_ok<T>(x, a.ldx, a.E, NV) && runs_ok<T>(dx, a.lddx, a.E, NV))
-    moe_route_bwd_kernel<T, LANES, NV, true><<<grid, ROUTE_THREADS, 0, st>>>(x, dx, a);
-  else
-    moe_route_bwd_kernel<T, LANES, NV, false><<<grid, ROUTE_THREADS, 0, st>>>(x, dx, a);
-  return launch_status("moe_route_bwd_kernel");
+  auto k = runs_ok<T>(x, a.ldx, a.E, NV) && runs_ok<T>(dx, a.lddx, a.E, NV)
+               ? moe_route_bwd_kernel<T, LANES, NV, true>
+               : moe_route_bwd_kernel<T, LANES, NV, false>;
+  return launch_overlapped("moe_route_bwd_kernel", k, dim3(grid), ROUTE_THREADS, 0, 0, st, x, dx,
+                           a);
 }
 template <typename T>
 int route_bwd_dispatch(const T* x, T* dx, const RouteBwdArgs& a, cudaStream_t st) {
