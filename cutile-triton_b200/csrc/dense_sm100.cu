@@ -20,6 +20,7 @@
 #include "sm100_ptx.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
@@ -761,32 +762,34 @@ static bool rows16(const void* p, int64_t ld, int rows) {
 }
 
 // ---- which kernel, tile and split ------------------------------------------------------
-// A model of the two kernels' times in microseconds, fitted to 965 runs: 91
-// products of 1 to 1536 rows, 640 to 14336 columns and 512 to 14336 k, each with
-// every tile and split (8% off a time; the choice by it takes 1.9% longer than
-// the best one measured, 14% at worst). A split CTA takes its k-blocks at 80 GB/s
-// when alone on its SM, two together at 150; 256 CTAs in clusters are sure to be
-// resident at once. A pair takes 0.3 us a k-block and 3 us a tile.
+// A model of the two kernels' times in microseconds. Its numbers make the choice
+// by it the fastest one measured as nearly as possible over 965 runs (91 products
+// of 1 to 1536 rows, 640 to 14336 columns, 512 to 14336 k, each with every tile
+// and split): it takes 0.5% longer than the best, 6% at worst. A split CTA takes
+// its k-blocks at 80 GB/s, alone or beside another on its SM; 256 CTAs in clusters
+// are sure to be resident at once, 296 single ones; more row tiles read the
+// weight again, mostly from L2. A pair takes 0.3 us a k-block and 2.5 us a tile.
 struct Plan {
   int BN, S;  // BN = 0: the pair kernel
 };
 
-static double split_us(const Product& p, int BN, int S, int sms, double moved) {
-  const int64_t tiles = (int64_t)((p.cols + SP_COLS - 1) / SP_COLS) * ((p.rows + BN - 1) / BN);
-  const int64_t ctas = tiles * S;
+static double split_us(const Product& p, int BN, int S, int sms, double out_bytes) {
+  const double tiles_r = (p.rows + BN - 1) / BN;
+  const double ctas = (double)((p.cols + SP_COLS - 1) / SP_COLS) * tiles_r * S;
   const int kb = (p.depth + BK - 1) / BK, per = (kb + S - 1) / S;
-  const double waves = (double)((ctas + 2 * sms - 1) / (2 * sms));
+  const double waves = std::ceil(ctas / (2 * sms));
   const double both = ctas > sms ? 2 : 1;
-  const double bytes = (double)per * sp_stage_bytes(BN);
-  const double load = waves * std::max(bytes / 80e3, both * bytes / 150e3);
-  return 2.7 + std::max(load, moved / 6.4e6) + waves * both * BN * 0.03 + (S > 1 ? 0.7 : 0) +
-         0.28 * S;
+  const double load = waves * per * sp_stage_bytes(BN) / 81.5e3;
+  const double moved = std::pow(tiles_r, 0.42) * 2.0 * p.cols * p.depth + 2.0 * p.rows * p.depth +
+                       out_bytes;
+  return 1.3 + std::max(load, moved / 9.56e6) + waves * both * BN * 0.036 + (S > 1 ? 0.93 : 0) +
+         0.31 * S;
 }
-static double pair_us(const Product& p, int pairs, double moved) {
-  const int64_t tiles = (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
+static double pair_us(const Product& p, int pairs, double out_bytes) {
+  const double tiles = (double)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
   const int kb = (p.depth + BK - 1) / BK;
-  const double waves = (double)((tiles + pairs - 1) / pairs);
-  return 4 + std::max(waves * (3 + 0.3 * kb), moved / 4.7e6);
+  const double moved = 2.0 * p.cols * p.depth + 2.0 * p.rows * p.depth + out_bytes;
+  return 3.7 + std::max(std::ceil(tiles / pairs) * (2.5 + 0.3 * kb), moved / 4.56e6);
 }
 
 // CTB_DENSE_PAIR=0 never takes the pair kernel, =1 whenever a pair can be resident.
@@ -799,11 +802,9 @@ static int pair_mode() {
 }
 
 static Plan choose_plan(const Product& p, int sms, int pairs) {
-  const double out = 1 + (p.Z ? 1 : 0) + (p.R ? 1 : 0);
-  const double moved = 2 * ((double)p.cols * p.depth + (double)p.rows * p.depth +
-                            out * (double)p.rows * p.cols);
+  const double out_bytes = (1 + (p.Z ? 1 : 0) + (p.R ? 1 : 0)) * 2.0 * p.rows * p.cols;
   Plan best = {0, 1};
-  double us = pairs > 0 ? pair_us(p, pairs, moved) : 1e30;
+  double us = pairs > 0 ? pair_us(p, pairs, out_bytes) : 1e30;
   const int mode = pair_mode();
   if (mode == 1 && pairs > 0) return best;
   if (mode == 0) us = 1e30;
@@ -815,7 +816,7 @@ static Plan choose_plan(const Product& p, int sms, int pairs) {
     for (int S = 1; S <= 8; ++S) {
       if (S > 1 && (S > kb / 2 || tiles_c * tiles_r * S > 256)) break;
       if (S == 5 || S == 7) continue;
-      const double t = split_us(p, BN, S, sms, moved);
+      const double t = split_us(p, BN, S, sms, out_bytes);
       if (t < us) {
         us = t;
         best = {BN, S};
