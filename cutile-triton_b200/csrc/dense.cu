@@ -50,42 +50,61 @@ bool tma_lines(const void* p, int64_t ld, int64_t lines) {
 }
 int64_t packed_bytes(int64_t lines, int64_t len) { return round256(2 * lines * round8(len)); }
 
-// Copies lines of 16-bit elements to lines round8(len) apart. One thread per 16
-// bytes of the result.
-__global__ void __launch_bounds__(256)
-    pack_kernel(const uint16_t* __restrict__ src, uint4* __restrict__ dst, int64_t lines, int len,
-                int64_t ld) {
+// Copies lines of 16-bit elements to lines round8(len) apart; one thread per 16
+// bytes of the result. Both operands of a product in one launch (the grid's y).
+// 4097 x 8193: 26 us for 134 MB moved (20 us at the copy rate).
+struct Pack {
+  const uint16_t* src;
+  uint4* dst;
+  int64_t lines, ld;
+  int len;
+};
+__global__ void __launch_bounds__(256) pack_kernel(const Pack first, const Pack second) {
   let_next_start();
   wait_for_previous();
-  const int runs = (len + 7) / 8;
-  const int64_t total = lines * runs;
+  const Pack& k = blockIdx.y ? second : first;
+  const int runs = (k.len + 7) / 8;
+  const int64_t total = k.lines * runs;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * 256) {
     const int64_t l = i / runs;
     const int c = (int)(i - l * runs) * 8;
-    const uint16_t* p = src + l * ld + c;
+    const uint16_t* p = k.src + l * k.ld + c;
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = c + 2 * j < len ? p[2 * j] : 0, hi = c + 2 * j + 1 < len ? p[2 * j + 1] : 0;
+      const uint32_t lo = c + 2 * j < k.len ? p[2 * j] : 0;
+      const uint32_t hi = c + 2 * j + 1 < k.len ? p[2 * j + 1] : 0;
       w[j] = lo | hi << 16;
     }
-    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    k.dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-// Replaces an operand that TMA cannot address by its copy at `ws`, which moves on.
-int pack_operand(const void** p, int64_t* ld, int64_t lines, int64_t len, uint8_t** ws, int sms,
-                 cudaStream_t st) {
-  if (lines == 0 || len == 0 || tma_lines(*p, *ld, lines)) return CTB_OK;
-  const int64_t grid = std::min<int64_t>((lines * ((len + 7) / 8) + 255) / 256, 16ll * sms);
-  const int rc = launch_overlapped("pack_kernel", pack_kernel, dim3((unsigned)grid), 256, 0, 0, st,
-                                   static_cast<const uint16_t*>(*p), reinterpret_cast<uint4*>(*ws),
-                                   lines, (int)len, *ld);
-  *p = *ws;
-  *ld = round8(len);
-  *ws += packed_bytes(lines, len);
-  return rc;
+// An operand of `lines` lines of `len` elements, and its replacement by a copy
+// in the workspace where TMA cannot address it.
+struct Operand {
+  const void** p;
+  int64_t* ld;
+  int64_t lines, len;
+};
+int pack_operands(Operand a, Operand b, uint8_t* ws, int sms, cudaStream_t st) {
+  Pack k[2] = {};
+  int n = 0;
+  int64_t most = 0;
+  for (const Operand& o : {a, b}) {
+    if (o.lines == 0 || o.len == 0 || tma_lines(*o.p, *o.ld, o.lines)) continue;
+    k[n++] = {static_cast<const uint16_t*>(*o.p), reinterpret_cast<uint4*>(ws), o.lines, *o.ld,
+              (int)o.len};
+    most = std::max(most, o.lines * ((o.len + 7) / 8));
+    *o.p = ws;
+    *o.ld = round8(o.len);
+    ws += packed_bytes(o.lines, o.len);
+  }
+  if (n == 0) return CTB_OK;
+  const int64_t grid = std::min<int64_t>((most + 255) / 256, 16ll * sms);
+  return launch_overlapped("pack_kernel", pack_kernel, dim3((unsigned)grid, n), 256, 0, 0, st, k[0],
+                           k[1]);
 }
 
 template <typename T>
@@ -266,13 +285,14 @@ int dense_bwd(const T* dC, const T* A, const T* B, const T* Z, T* dA, T* dB, flo
       if (rc) return rc;
     }
   }
+  const void *qA = A, *qB = B;
+  if (int rc = pack_operands({&qA, &lda, dB ? K : 0, M}, {&qB, &ldb, dA ? N : 0, K}, ws, sms, st))
+    return rc;
   if (dB && N > 0 && K > 0) {
-    const void* q = A;
-    if (int rc = pack_operand(&q, &lda, K, M, &ws, sms, st)) return rc;
     Product p = {};
     p.P = dZ;
     p.ldp = lddz;
-    p.Q = q;
+    p.Q = qA;
     p.ldq = lda;
     p.D = dB;
     p.ldd = lddb;
@@ -282,10 +302,8 @@ int dense_bwd(const T* dC, const T* A, const T* B, const T* Z, T* dA, T* dB, flo
     if (int rc = product<T>(p, sms, st)) return rc;
   }
   if (dA && M > 0 && K > 0) {
-    const void* q = B;
-    if (int rc = pack_operand(&q, &ldb, N, K, &ws, sms, st)) return rc;
     Product p = {};
-    p.P = q;
+    p.P = qB;
     p.ldp = ldb;
     p.p_mn = true;
     p.Q = dZ;
@@ -376,8 +394,8 @@ extern "C" int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const 
   p.ldz = ldz;
   auto st = static_cast<cudaStream_t>(stream);
   auto* ws = static_cast<uint8_t*>(workspace);
-  if (int rc = dense::pack_operand(&p.P, &p.ldp, N, K, &ws, pr.sm_count, st)) return rc;
-  if (int rc = dense::pack_operand(&p.Q, &p.ldq, K, M, &ws, pr.sm_count, st)) return rc;
+  if (int rc = dense::pack_operands({&p.P, &p.ldp, N, K}, {&p.Q, &p.ldq, K, M}, ws, pr.sm_count, st))
+    return rc;
   return dtype == CTB_F16 ? dense::product<__half>(p, pr.sm_count, st)
                           : dense::product<__nv_bfloat16>(p, pr.sm_count, st);
 }

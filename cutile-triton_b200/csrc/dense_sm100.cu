@@ -31,7 +31,7 @@ namespace dense {
 constexpr unsigned ERR_BIT = 64u;
 constexpr int BK = 64;  // k-block: one 128-byte swizzled row of 16-bit elements
 
-// ---- epilogue of 8 neighbouring columns of one row ---------------------------------
+// ---- epilogue -------------------------------------------------------------------------
 struct Epilogue {
   const void* bias;
   const void* R;
@@ -49,13 +49,15 @@ __device__ __forceinline__ void activate8(float (&z)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; i += 2) activate2<ACT>(z[i], z[i + 1]);
 }
+// 8 neighbouring columns of one row, of matrices whose rows are 16-byte runs; the
+// last run of a row may be short.
 template <typename T>
 __device__ __forceinline__ void finish8(const Epilogue& e, int64_t r, int c, float (&z)[8],
                                         const float (&bias)[8]) {
   const int n = min(8, e.cols - c);
 #pragma unroll
   for (int i = 0; i < 8; ++i) z[i] += bias[i];
-  const bool whole = e.vec && n == 8;
+  const bool whole = n == 8;
   if (e.Z) {
     T* zp = static_cast<T*>(e.Z) + r * e.ldz + c;
     if (whole) {
@@ -96,6 +98,14 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t r, int c, flo
   }
 }
 
+// One element, its bias added, and its residual.
+template <typename T>
+__device__ __forceinline__ void finish1(const Epilogue& e, int64_t r, int c, float z,
+                                        float residual) {
+  if (e.Z) from_f32(static_cast<T*>(e.Z) + r * e.ldz + c, z);
+  from_f32(static_cast<T*>(e.D) + r * e.ldd + c, activate_any(z, e.act) + residual);
+}
+
 template <typename T> struct Format;
 template <> struct Format<__half> {
   static constexpr uint32_t idesc = 0;
@@ -127,6 +137,11 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                : "r"(addr)
                : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t cluster_nctarank() {
@@ -250,15 +265,18 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
     }
     mma_commit_elect(done);
   }
-  // A thread's columns are the same for all its rows: 16 runs of 8 in a row, and
-  // the threads of the cluster a multiple of 16.
-  const int c = (int)(threadIdx.x % (SP_COLS / 8)) * 8;
+  // A thread's columns are the same for all its rows: 8 neighbours of one of 16
+  // runs, or (rows that are no 16-byte runs) lane, lane + 32, ...
+  const int c = a.e.vec ? (int)(threadIdx.x % (SP_COLS / 8)) * 8 : lane;
+  const int step = a.e.vec ? 1 : 32;
   float bias[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    bias[i] = !a.e.bias || c0 + c + i >= a.e.cols ? 0.f
-              : a.e.bias_f32 ? static_cast<const float*>(a.e.bias)[c0 + c + i]
-                             : to_f32(static_cast<const T*>(a.e.bias)[c0 + c + i]);
+  for (int i = 0; i < 8; ++i) {
+    const int64_t at = (int64_t)c0 + c + i * step;
+    bias[i] = !a.e.bias || at >= a.e.cols || (!a.e.vec && i >= SP_COLS / 32) ? 0.f
+              : a.e.bias_f32 ? static_cast<const float*>(a.e.bias)[at]
+                             : to_f32(static_cast<const T*>(a.e.bias)[at]);
+  }
   // All roles meet at the finished accumulator. It exists on the way out of a
   // wait that gave up too; the host is told by the error word.
   mbar_wait_bounded(done, 0, abort_flag, ERR_BIT);
@@ -292,8 +310,48 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
 
   const uint32_t mine = smem_u32(partial);
   const int live_rows = (int)min((int64_t)BN, a.e.rows - r0);
+  if (!a.e.vec) {
+    // A warp per row, so that the 2-byte accesses of a row stay together, four
+    // rows' residuals asked for at a time.
+    constexpr int WARPS = SP_THREADS / 32, FLIGHT = 4, EACH = SP_COLS / 32;
+    for (int rb = (int)rank * WARPS + warp; rb < live_rows; rb += (int)S * WARPS * FLIGHT) {
+      T res[FLIGHT][EACH];
+      if (a.e.R) {
+#pragma unroll
+        for (int j = 0; j < FLIGHT; ++j)
+#pragma unroll
+          for (int i = 0; i < EACH; ++i) {
+            const int r = rb + j * (int)S * WARPS, col = c0 + i * 32 + lane;
+            if (r < live_rows && col < a.e.cols)
+              res[j][i] = static_cast<const T*>(a.e.R)[(r0 + r) * a.e.ldr + col];
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < FLIGHT; ++j) {
+        const int r = rb + j * (int)S * WARPS;
+        if (r >= live_rows) break;
+        float z[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) z[i] = 0.f;
+        for (uint32_t s = 0; s < S; ++s) {
+          const int at = r * SP_COLS + lane;
+          const uint32_t from = mapa_shared(mine, s) + (uint32_t)at * 4;
+#pragma unroll
+          for (int i = 0; i < EACH; ++i)
+            z[i] += s == rank ? partial[at + i * 32] : ld_cluster_f1(from + i * 128);
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const int col = c0 + i * 32 + lane;
+          if (col < a.e.cols)
+            finish1<T>(a.e, r0 + r, col, z[i] + bias[i], a.e.R ? to_f32(res[j][i]) : 0.f);
+        }
+      }
+    }
+  }
   for (int r = (int)(rank * SP_THREADS + threadIdx.x) / (SP_COLS / 8);
-       r < live_rows && c0 + c < a.e.cols; r += (int)S * (SP_THREADS / (SP_COLS / 8))) {
+       a.e.vec && r < live_rows && c0 + c < a.e.cols;
+       r += (int)S * (SP_THREADS / (SP_COLS / 8))) {
     float z[8] = {};
     for (uint32_t s = 0; s < S; ++s) {
       float4 lo, hi;
