@@ -821,12 +821,12 @@ static bool rows16(const void* p, int64_t ld, int rows) {
 
 // ---- which kernel, tile and split ------------------------------------------------------
 // A model of the two kernels' times in microseconds. Its numbers make the choice
-// by it the fastest one measured as nearly as possible over 965 runs (91 products
-// of 1 to 1536 rows, 640 to 14336 columns, 512 to 14336 k, each with every tile
-// and split): it takes 0.5% longer than the best, 6% at worst. A split CTA takes
-// its k-blocks at 80 GB/s, alone or beside another on its SM; 256 CTAs in clusters
-// are sure to be resident at once, 296 single ones; more row tiles read the
-// weight again, mostly from L2. A pair takes 0.3 us a k-block and 2.5 us a tile.
+// by it the fastest one measured as nearly as possible over 1658 runs (150
+// products of 1 to 6000 rows, 256 to 14336 columns, 300 to 14336 k, each with
+// every tile and split): it takes 1.5% longer than the best, 18% at worst. A split
+// CTA takes its k-blocks at 80 GB/s, alone or beside another on its SM; 256 CTAs
+// in clusters are sure to be resident at once, 296 single ones; more row tiles
+// read the weight again from L2. A pair takes 0.3 us a k-block and 3.2 us a tile.
 struct Plan {
   int BN, S;  // BN = 0: the pair kernel
 };
@@ -837,17 +837,17 @@ static double split_us(const Product& p, int BN, int S, int sms, double out_byte
   const int kb = (p.depth + BK - 1) / BK, per = (kb + S - 1) / S;
   const double waves = std::ceil(ctas / (2 * sms));
   const double both = ctas > sms ? 2 : 1;
-  const double load = waves * per * sp_stage_bytes(BN) / 81.5e3;
-  const double moved = std::pow(tiles_r, 0.42) * 2.0 * p.cols * p.depth + 2.0 * p.rows * p.depth +
+  const double load = waves * per * sp_stage_bytes(BN) / 79.7e3;
+  const double moved = std::pow(tiles_r, 0.84) * 2.0 * p.cols * p.depth + 2.0 * p.rows * p.depth +
                        out_bytes;
-  return 1.3 + std::max(load, moved / 9.56e6) + waves * both * BN * 0.036 + (S > 1 ? 0.93 : 0) +
-         0.31 * S;
+  return 2.25 + std::max(load, moved / 14.5e6) + waves * both * BN * 0.032 + (S > 1 ? 0.28 : 0) +
+         0.33 * S;
 }
 static double pair_us(const Product& p, int pairs, double out_bytes) {
   const double tiles = (double)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
   const int kb = (p.depth + BK - 1) / BK;
   const double moved = 2.0 * p.cols * p.depth + 2.0 * p.rows * p.depth + out_bytes;
-  return 3.7 + std::max(std::ceil(tiles / pairs) * (2.5 + 0.3 * kb), moved / 4.56e6);
+  return 3.6 + std::max(std::ceil(tiles / pairs) * (3.2 + 0.304 * kb), moved / 4.43e6);
 }
 
 // CTB_DENSE_PAIR=0 never takes the pair kernel, =1 whenever a pair can be resident.
