@@ -133,6 +133,9 @@ int moe_take_device_error(unsigned int* out);
 int layernorm_bwd_take_device_error(unsigned int* out);
 int selftest_take_device_error(unsigned int* out);
 int dense_take_device_error(unsigned int* out);
+namespace dense {
+int device_setup(int* pairs);
+}
 }
 
 extern "C" int ctb_init(int device) {
@@ -148,6 +151,8 @@ extern "C" int ctb_init(int device) {
   int rc = current_props(&p);
   if (rc == CTB_OK) rc = gemm_device_setup();
   if (rc == CTB_OK) rc = fmha_device_setup();
+  int pairs = 0;
+  if (rc == CTB_OK) rc = dense::device_setup(&pairs);
   cudaSetDevice(prev);
   return rc;
 }

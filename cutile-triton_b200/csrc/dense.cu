@@ -228,14 +228,14 @@ __global__ void __launch_bounds__(256)
 
 // Spans of the rows: 32 rows at least, at most what gives SLOPE_CTAS CTAs.
 int spans_of(int N, int M) {
-  const int strips = std::max(1, (M + 255) / 256);
-  return std::max(1, std::min((N + 31) / 32, SLOPE_CTAS / strips));
+  const int64_t strips = std::max<int64_t>(1, ((int64_t)M + 255) / 256);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)N + 31) / 32, SLOPE_CTAS / strips));
 }
 
 template <typename T, int W>
 int slope_launch(const T* dC, const T* Z, T* dZ, float* sums, int N, int M, int64_t lddc,
                  int64_t ldz, int64_t lddz, int act, int spans, cudaStream_t st) {
-  const dim3 grid((M + 32 * W - 1) / (32 * W), spans);
+  const dim3 grid((unsigned)(((int64_t)M + 32 * W - 1) / (32 * W)), spans);
   auto k = slope_kernel<T, W, CTB_ACT_NONE>;
   switch (act) {
     case CTB_ACT_RELU: k = slope_kernel<T, W, CTB_ACT_RELU>; break;
@@ -245,7 +245,7 @@ int slope_launch(const T* dC, const T* Z, T* dZ, float* sums, int N, int M, int6
     default: break;
   }
   return launch_overlapped("slope_kernel", k, grid, SLOPE_THREADS, 0, 0, st, dC, Z, dZ, sums, N, M,
-                           lddc, ldz, lddz, (N + spans - 1) / spans);
+                           lddc, ldz, lddz, (int)(((int64_t)N + spans - 1) / spans));
 }
 
 // dZ goes to the workspace where it is not dC itself: with an activation, or
@@ -280,7 +280,8 @@ int dense_bwd(const T* dC, const T* A, const T* B, const T* Z, T* dA, T* dB, flo
                   : slope_launch<T, 1>(dC, Z, dz, sums, N, M, lddc, ldz, lddz, act, spans, st);
     if (rc) return rc;
     if (dbias && spans > 1) {
-      rc = launch_overlapped("fold_kernel", fold_kernel, dim3((M + 31) / 32), 256, 0, 0, st, sums,
+      rc = launch_overlapped("fold_kernel", fold_kernel, dim3((unsigned)(((int64_t)M + 31) / 32)), 256, 0, 0,
+                             st, sums,
                              dbias, M, spans);
       if (rc) return rc;
     }
@@ -368,6 +369,7 @@ extern "C" int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const 
     return set_error(CTB_ERR_LAYOUT, "dense: leading dimension smaller than the column length");
   if (M == 0 || N == 0) return CTB_OK;
   if (!C || (K > 0 && (!A || !B))) return set_error(CTB_ERR_ARG, "dense: NULL pointer");
+  if (Z && (Z == C || Z == R)) return set_error(CTB_ERR_ARG, "dense: Z must be a matrix of its own");
   const int64_t need = ctb_dense_fwd_workspace_bytes(A, B, M, N, K, lda, ldb);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return set_error(CTB_ERR_ARG, "dense: the workspace needs " + std::to_string(need) +

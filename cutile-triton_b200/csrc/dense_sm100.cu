@@ -832,9 +832,9 @@ struct Plan {
 };
 
 static double split_us(const Product& p, int BN, int S, int sms, double out_bytes) {
-  const double tiles_r = (p.rows + BN - 1) / BN;
-  const double ctas = (double)((p.cols + SP_COLS - 1) / SP_COLS) * tiles_r * S;
-  const int kb = (p.depth + BK - 1) / BK, per = (kb + S - 1) / S;
+  const double tiles_r = (double)(((int64_t)p.rows + BN - 1) / BN);
+  const double ctas = (double)(((int64_t)p.cols + SP_COLS - 1) / SP_COLS) * tiles_r * S;
+  const int kb = (int)(((int64_t)p.depth + BK - 1) / BK), per = (kb + S - 1) / S;
   const double waves = std::ceil(ctas / (2 * sms));
   const double both = ctas > sms ? 2 : 1;
   const double load = waves * per * sp_stage_bytes(BN) / 79.7e3;
@@ -844,8 +844,8 @@ static double split_us(const Product& p, int BN, int S, int sms, double out_byte
          0.33 * S;
 }
 static double pair_us(const Product& p, int pairs, double out_bytes) {
-  const double tiles = (double)((p.rows + 255) / 256) * ((p.cols + 255) / 256);
-  const int kb = (p.depth + BK - 1) / BK;
+  const double tiles = (double)(((int64_t)p.rows + 255) / 256 * (((int64_t)p.cols + 255) / 256));
+  const int kb = (int)(((int64_t)p.depth + BK - 1) / BK);
   const double moved = 2.0 * p.cols * p.depth + 2.0 * p.rows * p.depth + out_bytes;
   return 3.6 + std::max(std::ceil(tiles / pairs) * (3.2 + 0.304 * kb), moved / 4.43e6);
 }
@@ -866,10 +866,10 @@ static Plan choose_plan(const Product& p, int sms, int pairs) {
   const int mode = pair_mode();
   if (mode == 1 && pairs > 0) return best;
   if (mode == 0) us = 1e30;
-  const int64_t tiles_c = (p.cols + SP_COLS - 1) / SP_COLS;
-  const int kb = (p.depth + BK - 1) / BK;
+  const int64_t tiles_c = ((int64_t)p.cols + SP_COLS - 1) / SP_COLS;
+  const int kb = (int)(((int64_t)p.depth + BK - 1) / BK);
   for (int BN = p.p_mn ? 64 : 16; BN <= 128; BN *= 2) {
-    const int64_t tiles_r = (p.rows + BN - 1) / BN;
+    const int64_t tiles_r = ((int64_t)p.rows + BN - 1) / BN;
     if (tiles_r > 65535 && !(BN == 128 && us >= 1e30)) continue;  // the grid's y
     for (int S = 1; S <= 8; ++S) {
       if (S > 1 && (S > kb / 2 || tiles_c * tiles_r * S > 256)) break;
@@ -892,8 +892,8 @@ int split_launch(const Product& p, const Epilogue& e, int S, cudaStream_t st) {
   if (int rc = operand_map<T>(&tmP, p.P, p.ldp, P_MN, p.rows, p.depth, BN)) return rc;
   SplitArgs a;
   a.e = e;
-  a.num_kb = (p.depth + BK - 1) / BK;
-  const int64_t tiles_c = (p.cols + SP_COLS - 1) / SP_COLS, tiles_r = ((int64_t)p.rows + BN - 1) / BN;
+  a.num_kb = (int)(((int64_t)p.depth + BK - 1) / BK);
+  const int64_t tiles_c = ((int64_t)p.cols + SP_COLS - 1) / SP_COLS, tiles_r = ((int64_t)p.rows + BN - 1) / BN;
   if (tiles_r > 65535) return set_error(CTB_ERR_SHAPE, "dense: too many rows");
   return launch_overlapped("product_split_kernel", product_split_kernel<T, Q_MN, P_MN, BN>,
                            dim3((unsigned)(tiles_c * S), (unsigned)tiles_r), SP_THREADS,
@@ -909,7 +909,7 @@ int box_map(CUtensorMap* m, const void* base, int64_t ld, int rows, int cols, bo
     return CTB_OK;
   }
   const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows};
-  const uint64_t strides[1] = {(uint64_t)(rows > 1 ? ld : (cols + 7) / 8 * 8) * 2};
+  const uint64_t strides[1] = {(uint64_t)(rows > 1 ? ld : ((int64_t)cols + 7) / 8 * 8) * 2};
   const uint32_t box[2] = {32, 32};
   return encode_tmap(m, Format<T>::map, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
@@ -927,9 +927,9 @@ int pair_launch(const Product& p, const Epilogue& e, int pairs, cudaStream_t st)
   if (int rc = box_map<T>(&tmD, p.D, p.ldd, p.rows, p.cols, a.d_tma)) return rc;
   if (int rc = box_map<T>(&tmZ, p.Z, p.ldz, p.rows, p.cols, a.z_tma)) return rc;
   if (int rc = box_map<T>(&tmR, p.R, p.ldr, p.rows, p.cols, a.r_tma)) return rc;
-  a.num_kb = (p.depth + BK - 1) / BK;
-  a.tiles_r = (p.rows + 255) / 256;
-  a.tiles_c = (p.cols + 255) / 256;
+  a.num_kb = (int)(((int64_t)p.depth + BK - 1) / BK);
+  a.tiles_r = (int)(((int64_t)p.rows + 255) / 256);
+  a.tiles_c = (int)(((int64_t)p.cols + 255) / 256);
   a.num_tiles = (int64_t)a.tiles_r * a.tiles_c;
   return launch_overlapped("product_pair_kernel", product_pair_kernel<T, P_MN, Q_MN>,
                            dim3((unsigned)(2 * std::min<int64_t>(a.num_tiles, pairs))), PR_THREADS,
@@ -944,8 +944,8 @@ int product_sm100(const Product& p0, int sms, cudaStream_t st) {
   if (int rc = device_setup(&pairs)) return rc;
   Product p = p0;
   // The distance between lines does not matter where there is one: any that TMA takes.
-  if ((p.p_mn ? p.depth : p.rows) == 1) p.ldp = ((p.p_mn ? p.rows : p.depth) + 7) / 8 * 8;
-  if ((p.q_mn ? p.depth : p.cols) == 1) p.ldq = ((p.q_mn ? p.cols : p.depth) + 7) / 8 * 8;
+  if ((p.p_mn ? p.depth : p.rows) == 1) p.ldp = ((int64_t)(p.p_mn ? p.rows : p.depth) + 7) / 8 * 8;
+  if ((p.q_mn ? p.depth : p.cols) == 1) p.ldq = ((int64_t)(p.q_mn ? p.cols : p.depth) + 7) / 8 * 8;
   Epilogue e;
   e.bias = p.bias;
   e.R = p.R;

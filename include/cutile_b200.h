@@ -313,7 +313,7 @@ typedef enum {
  * R and Z are M x N; lda, ldb, ldr, ldz, ldc are column strides. bias: M
  * elements of dtype bias_dtype (the matrices' or F32), or NULL; R (residual)
  * may be NULL, and may be C itself; Z receives the value before the activation (what
- * ctb_dense_bwd needs), or NULL. Sums, bias, activation and residual are
+ * ctb_dense_bwd needs), or NULL. Nothing else may overlap what is written. Sums, bias, activation and residual are
  * Float32, rounded once to C (and once to Z). The result of a call does not
  * depend on the schedule (no atomics). `workspace` (16-byte aligned) of at
  * least ctb_dense_fwd_workspace_bytes() bytes, which is 0 when A and B start

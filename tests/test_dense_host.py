@@ -44,7 +44,8 @@ def test_oracle_gradients_against_differences(act):
     (dict(act=5), -1), (dict(act=-1), -1), (dict(bias=NP, bd=_lib.CTB_BF16), -2),
     (dict(bias=NP, bd=_lib.CTB_F64), -2), (dict(lda=15), -4), (dict(ldb=31), -4),
     (dict(ldc=15), -4), (dict(R=NP, ldr=15), -4), (dict(Z=NP, ldz=15), -4), (dict(A=None), -1),
-    (dict(B=None), -1), (dict(C=None), -1), (dict(M=0, A=None, C=None), 0),
+    (dict(B=None), -1), (dict(C=None), -1), (dict(Z=NP), -1), (dict(Z=NP + 64, R=NP + 64), -1),
+    (dict(M=0, A=None, C=None), 0),
     (dict(N=0, B=None, C=None), 0),
 ])
 def test_dense_refusals(kw, code):
