@@ -26,7 +26,8 @@ using Libdl
 import cuTile as ct
 
 export triton_kernel, triton_kernel_candidates, launch!, install_shim!, use_b200!, B200Kernel,
-       softmax_host!, layernorm_fwd_host!, vadd_host!, moe_align
+       softmax_host!, layernorm_fwd_host!, vadd_host!, moe_align,
+       dense!, dense_bwd!, moe_route, moe_route_bwd, moe_combine!, moe_combine_bwd
 
 # ---------------------------------------------------------------------------- library
 const LIBPATH = Ref{String}("")
@@ -328,6 +329,135 @@ function moe_align(topk_ids::CuMatrix{Int32}, num_experts::Integer; block::Integ
                 topk_ids, n, num_experts, block, sorted, experts, ntp, cap,
                 CUDA.stream().handle))
     return sorted, experts, ntp
+end
+
+# ---------------------------------------------------------------------------- layer calls
+const F16s = Union{Float16,Core.BFloat16}
+const ACTS = Dict(:none => 0, :relu => 1, :gelu => 2, :gelu_tanh => 3, :silu => 4)
+const SCORES = Dict(:softmax => 0, :sigmoid => 1)
+ldim(x) = stride(x, 2)
+orC(x) = x === nothing ? CU_NULL : pointer(x)
+codeof(::Type{Float16}) = Int32(1)
+codeof(::Type{Core.BFloat16}) = Int32(2)
+codeof(::Type{Float32}) = Int32(3)
+
+"""
+    dense!(C, A, B; bias=nothing, act=:none, R=nothing, Z=nothing)
+
+C = act.(A * B .+ bias) .+ R for Float16 or BFloat16 columns: A (M, K) the
+weight, B (K, N) a column per token; `act` one of :none, :relu, :gelu,
+:gelu_tanh, :silu; bias of the matrices' type or Float32; Z receives the value
+before the activation (`ctb_dense_fwd`).
+"""
+function dense!(C::StridedCuMatrix{T}, A::StridedCuMatrix{T}, B::StridedCuMatrix{T}; bias=nothing,
+                act::Symbol=:none, R=nothing, Z=nothing) where {T<:F16s}
+    M, K = size(A)
+    N = size(B, 2)
+    size(B, 1) == K && size(C) == (M, N) || error("b200: dense!: sizes disagree")
+    nws = ccall(sym(:ctb_dense_fwd_workspace_bytes), Int64,
+                (CuPtr{T}, CuPtr{T}, Int32, Int32, Int32, Int64, Int64), A, B, M, N, K, ldim(A), ldim(B))
+    ws = CuArray{UInt8}(undef, max(nws, 1))
+    GC.@preserve A B C bias R Z ws check(ccall(sym(:ctb_dense_fwd), Cint,
+                (Int32, CuPtr{T}, CuPtr{T}, CuPtr{Cvoid}, Int32, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{T},
+                 Int32, Int32, Int32, Int64, Int64, Int64, Int64, Int64, Int32, CuPtr{UInt8}, Int64,
+                 Ptr{Cvoid}),
+                codeof(T), A, B, orC(bias), bias === nothing ? 0 : codeof(eltype(bias)), orC(R), orC(Z),
+                C, M, N, K, ldim(A), ldim(B), R === nothing ? 0 : ldim(R), Z === nothing ? 0 : ldim(Z),
+                ldim(C), ACTS[act], ws, nws, CUDA.stream().handle))
+    return C
+end
+
+"""
+    dense_bwd!(dA, dB, dbias, dC, A, B; act=:none, Z=nothing)
+
+Gradients of `dense!` from dC (M, N); any of dA (M, K), dB (K, N), dbias (M,
+Float32) may be `nothing`. Z is the forward call's (`ctb_dense_bwd`).
+"""
+function dense_bwd!(dA, dB, dbias, dC::StridedCuMatrix{T}, A::StridedCuMatrix{T}, B::StridedCuMatrix{T};
+                    act::Symbol=:none, Z=nothing) where {T<:F16s}
+    M, K = size(A)
+    N = size(B, 2)
+    size(B, 1) == K && size(dC) == (M, N) || error("b200: dense_bwd!: sizes disagree")
+    nws = ccall(sym(:ctb_dense_bwd_workspace_bytes), Int64,
+                (CuPtr{T}, CuPtr{T}, CuPtr{T}, Int32, Int32, Int32, Int64, Int64, Int64, Int32, Int32),
+                dC, A, B, M, N, K, ldim(dC), ldim(A), ldim(B), ACTS[act], dbias === nothing ? 0 : 1)
+    ws = CuArray{UInt8}(undef, max(nws, 1))
+    GC.@preserve dA dB dbias dC A B Z ws check(ccall(sym(:ctb_dense_bwd), Cint,
+                (Int32, CuPtr{T}, CuPtr{T}, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid},
+                 CuPtr{Cvoid}, Int32, Int32, Int32, Int64, Int64, Int64, Int64, Int64, Int64, Int32,
+                 CuPtr{UInt8}, Int64, Ptr{Cvoid}),
+                codeof(T), dC, A, B, orC(Z), orC(dA), orC(dB), orC(dbias), M, N, K, ldim(dC), ldim(A),
+                ldim(B), Z === nothing ? 0 : ldim(Z), dA === nothing ? 0 : ldim(dA),
+                dB === nothing ? 0 : ldim(dB), ACTS[act], ws, nws, CUDA.stream().handle))
+    return dA, dB, dbias
+end
+
+"""
+    moe_route(logits, topk; score=:softmax, bias, groups=1, topk_groups=groups, group_top=2,
+              renorm=true, scale=1) -> (weights, ids)
+
+Routes each column of the (E, T) logits to `topk` experts (`ctb_moe_route`):
+weights Float32 and 0-based ids Int32, both (topk, T), for `moe_align` and the
+`moe` kernel; id -1 where no expert is available.
+"""
+function moe_route(logits::StridedCuMatrix{T}, topk::Integer; score::Symbol=:softmax, bias=nothing,
+                   groups::Integer=1, topk_groups::Integer=groups, group_top::Integer=2,
+                   renorm::Bool=true, scale::Real=1) where {T<:Union{F16s,Float32}}
+    E, n = size(logits)
+    weights, ids = CuArray{Float32}(undef, topk, n), CuArray{Int32}(undef, topk, n)
+    GC.@preserve bias check(ccall(sym(:ctb_moe_route), Cint,
+                (Int32, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Float32}, CuPtr{Int32}, Int32, Int32, Int32, Int64,
+                 Int32, Int32, Int32, Int32, Int32, Float32, Ptr{Cvoid}),
+                codeof(T), logits, orC(bias), weights, ids, n, E, topk, ldim(logits), SCORES[score],
+                groups, topk_groups, group_top, renorm, scale, CUDA.stream().handle))
+    return weights, ids
+end
+
+"Gradient of `moe_route`'s weights with respect to the logits, for the ids it gave (`ctb_moe_route_bwd`)."
+function moe_route_bwd(dweights::CuMatrix{Float32}, logits::StridedCuMatrix{T}, ids::CuMatrix{Int32};
+                       score::Symbol=:softmax, renorm::Bool=true, scale::Real=1) where {T<:Union{F16s,Float32}}
+    E, n = size(logits)
+    size(ids, 2) == n && size(dweights) == size(ids) || error("b200: moe_route_bwd: sizes disagree")
+    dlogits = CuArray{T}(undef, E, n)
+    check(ccall(sym(:ctb_moe_route_bwd), Cint,
+                (Int32, CuPtr{Float32}, CuPtr{T}, CuPtr{Int32}, CuPtr{T}, Int32, Int32, Int32, Int64, Int64,
+                 Int32, Int32, Float32, Ptr{Cvoid}),
+                codeof(T), dweights, logits, ids, dlogits, n, E, size(ids, 1), ldim(logits), E,
+                SCORES[score], renorm, scale, CUDA.stream().handle))
+    return dlogits
+end
+
+"""
+    moe_combine!(out, y, topk; weights=nothing, ids=nothing, num_experts=0, R=nothing)
+
+out[:, t] = R[:, t] + sum over j of weights[j, t] * y[:, (t - 1) topk + j], slots
+with an id outside 0:num_experts-1 left out (`ctb_moe_combine`).
+"""
+function moe_combine!(out::StridedCuMatrix{T}, y::StridedCuMatrix{T}, topk::Integer; weights=nothing,
+                      ids=nothing, num_experts::Integer=0, R=nothing) where {T<:F16s}
+    N, n = size(out)
+    size(y) == (N, n * topk) || error("b200: moe_combine!: sizes disagree")
+    GC.@preserve weights ids R check(ccall(sym(:ctb_moe_combine), Cint,
+                (Int32, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{T}, Int32, Int32, Int32,
+                 Int32, Int64, Int64, Int64, Ptr{Cvoid}),
+                codeof(T), y, orC(weights), orC(ids), orC(R), out, n, topk, N, num_experts, ldim(y),
+                R === nothing ? 0 : ldim(R), ldim(out), CUDA.stream().handle))
+    return out
+end
+
+"Gradients (dy, dweights) of `moe_combine!` from dout (N, T) (`ctb_moe_combine_bwd`)."
+function moe_combine_bwd(dout::StridedCuMatrix{T}, y, topk::Integer; weights=nothing, ids=nothing,
+                         num_experts::Integer=0) where {T<:F16s}
+    N, n = size(dout)
+    dy = CuArray{T}(undef, N, n * topk)
+    dweights = weights === nothing ? nothing : CuArray{Float32}(undef, topk, n)
+    GC.@preserve y weights ids dweights check(ccall(sym(:ctb_moe_combine_bwd), Cint,
+                (Int32, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{T}, CuPtr{Cvoid}, Int32,
+                 Int32, Int32, Int32, Int64, Int64, Int64, Ptr{Cvoid}),
+                codeof(T), dout, weights === nothing ? CU_NULL : pointer(y), orC(weights), orC(ids), dy,
+                orC(dweights), n, topk, N, num_experts, ldim(dout), weights === nothing ? 0 : ldim(y), N,
+                CUDA.stream().handle))
+    return dy, dweights
 end
 
 "Initialises the library on the active CUDA device (kernel attributes, checks sm_100)."

@@ -312,12 +312,13 @@ typedef enum {
  * column-major: A is M x K (the weight), B is K x N (a column per token), C,
  * R and Z are M x N; lda, ldb, ldr, ldz, ldc are column strides. bias: M
  * elements of dtype bias_dtype (the matrices' or F32), or NULL; R (residual)
- * may be NULL, and may be C itself; Z receives the value before the activation (what
- * ctb_dense_bwd needs), or NULL. Nothing else may overlap what is written. Sums, bias, activation and residual are
- * Float32, rounded once to C (and once to Z). The result of a call does not
- * depend on the schedule (no atomics). `workspace` (16-byte aligned) of at
- * least ctb_dense_fwd_workspace_bytes() bytes, which is 0 when A and B start
- * on 16-byte boundaries and lda and ldb are multiples of 8. */
+ * may be NULL, and may be C itself; Z receives the value before the
+ * activation (what ctb_dense_bwd needs), or is NULL. Nothing else may overlap
+ * what is written. Sums, bias, activation and residual are Float32, rounded
+ * once to C (and once to Z); no atomics, so a call's result is always the
+ * same. `workspace` (16-byte aligned) of at least
+ * ctb_dense_fwd_workspace_bytes() bytes, which is 0 when A and B start on
+ * 16-byte boundaries and lda and ldb are multiples of 8. */
 int64_t ctb_dense_fwd_workspace_bytes(const void* A, const void* B, int32_t M, int32_t N,
                                       int32_t K, int64_t lda, int64_t ldb);
 int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const void* bias,
