@@ -161,6 +161,9 @@ struct RouteArgs {
   int T, E, topk;
   int64_t ldx;
   int sigmoid, groups, topk_groups, group_top, renorm;
+  int group_size;   // experts per group
+  int group_lanes;  // lanes per group where that is a power of two of whole lanes, else 0
+  bool bias_runs;   // the bias is made of whole runs of NV floats, 16-byte aligned
   float scale;
 };
 
@@ -195,18 +198,32 @@ __device__ __forceinline__ bool too_close_unbiased(float hi, float lo) {
   return !(hi > 1e-30f && hi - lo > 2.f * hi * (4e-6f + 2.5e-7f * fabsf(__logf(hi))));
 }
 
+// Whether the order between the kept groups (`in`) and the others is too close
+// for 32 bits; each lane holds a group's score and the magnitude of its terms.
+__device__ __forceinline__ bool groups_close(bool biased, bool counts, bool in, float score,
+                                             float magnitude) {
+  const uint32_t k = key_of(score);
+  const float lo = value_of(__reduce_min_sync(FULL, counts && in ? k : 0xffffffffu));
+  const float hi = value_of(__reduce_max_sync(FULL, counts && !in ? k : kNone32));
+  const float mag = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(magnitude)));
+  // A group without an expert (-inf) is not in doubt.
+  return hi > -INFINITY && (biased ? too_close_biased(lo, hi, mag) : too_close_unbiased(lo, hi));
+}
+
 // Keys of the experts outside the best topk_groups groups become 0 (c is -inf
-// where an expert is not available); returns
-// whether the choice between groups was too close for 32 bits. LANES == 32.
+// where an expert is not available); returns whether the choice between groups
+// was too close for 32 bits. LANES == 32.
 template <typename S, int NV>
 __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV],
                                             typename KeyOf<S>::type (&key)[NV], S* row) {
-  const int lane = threadIdx.x & 31, size = a.E / a.groups;
+  const int lane = threadIdx.x & 31, size = a.group_size;
   const S none = -INFINITY;
   S best = none, second = none;
-  const int span = size / NV;  // lanes per group
-  if (size % NV == 0 && (span & (span - 1)) == 0) {
-    // Whole lanes per group: the two best of a lane's registers, then of neighbours.
+  if (a.group_lanes > 0) {
+    // A power of two of whole lanes per group: the two best of a lane's
+    // registers, then of neighbours, so that every lane of a group knows its
+    // score. Its rank among the groups is counted by the group's lanes together.
+    const int span = a.group_lanes, part = lane & (span - 1), first = lane - part;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       second = max(second, min(best, c[v]));
@@ -217,66 +234,61 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV]
       second = max(max(second, s), min(best, b));
       best = max(best, b);
     }
-    const int from = min(lane * span, 31);
-    best = __shfl_sync(FULL, best, from);
-    second = __shfl_sync(FULL, second, from);
-  } else {
-    // Through shared memory; one word in 32 is skipped so that lanes that
-    // start a multiple of 32 apart use different banks.
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = lane * NV + v;
-      if (i < a.E) row[i + (i >> 5)] = c[v];
+    const S score = a.group_top > 1 && second > none ? best + second : best;
+    const bool counts = first < a.groups * span;  // lanes past the last expert have no group
+    int rank = 0;
+    for (int i = 0; i < a.groups; i += span) {
+      const int from = (i + part) * span;  // a lane of group i + part
+      const S o = __shfl_sync(FULL, score, min(from, 31));
+      rank += i + part < a.groups && (o > score || (o == score && from < first));
     }
-    __syncwarp();
-    if (lane < a.groups)
-      for (int i = lane * size; i < (lane + 1) * size; ++i) {
-        const S x = row[i + (i >> 5)];
-        second = max(second, min(best, x));
-        best = max(best, x);
-      }
-    __syncwarp();
+    for (int o = 1; o < span; o <<= 1) rank += __shfl_xor_sync(FULL, rank, o);
+    const bool in = rank < a.topk_groups;
+    if (!in) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) key[v] = 0;
+    }
+    if (sizeof(S) != 4) return false;
+    const float magnitude = !counts || !(best > none) ? 0.f
+                            : fabsf((float)best) + (second > none ? fabsf((float)second) : 0.f);
+    return groups_close(a.bias != nullptr, counts, in, (float)score, magnitude);
   }
-  S score = best;
-  if (a.group_top > 1 && second > none) score = best + second;
-  if (lane >= a.groups) score = none;
+  // Through shared memory, a lane per group; one word in 32 is skipped so that
+  // lanes that start a multiple of 32 apart use different banks.
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int i = lane * NV + v;
+    if (i < a.E) row[i + (i >> 5)] = c[v];
+  }
+  __syncwarp();
+  if (lane < a.groups)
+    for (int i = lane * size; i < (lane + 1) * size; ++i) {
+      const S x = row[i + (i >> 5)];
+      second = max(second, min(best, x));
+      best = max(best, x);
+    }
+  __syncwarp();
+  const S score = a.group_top > 1 && second > none ? best + second : best;
   int rank = 0;
   for (int g = 0; g < a.groups; ++g) {
     const S o = __shfl_sync(FULL, score, g);
     rank += o > score || (o == score && g < lane);
   }
-  const bool in = lane < a.groups && rank < a.topk_groups;
+  const bool counts = lane < a.groups, in = counts && rank < a.topk_groups;
   const unsigned kept = __ballot_sync(FULL, in);
-  if (size % NV == 0) {  // a lane's experts share a group
-    if (lane * NV < a.E && !(kept >> (lane * NV / size) & 1u)) {
+  int g = lane * NV / size, at = lane * NV - g * size;
 #pragma unroll
-      for (int v = 0; v < NV; ++v) key[v] = 0;
-    }
-  } else {
-    int g = lane * NV / size, at = lane * NV - g * size;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      if (lane * NV + v < a.E && !(kept >> g & 1u)) key[v] = 0;
-      if (++at == size) {
-        at = 0;
-        ++g;
-      }
+  for (int v = 0; v < NV; ++v) {
+    if (lane * NV + v < a.E && !(kept >> g & 1u)) key[v] = 0;
+    if (++at == size) {
+      at = 0;
+      ++g;
     }
   }
-  bool close = false;
-  if (sizeof(S) == 4) {
-    const uint32_t k = key_of((float)score);
-    const float lo = value_of(__reduce_min_sync(FULL, in ? k : 0xffffffffu));
-    const float hi = value_of(__reduce_max_sync(FULL, lane < a.groups && !in ? k : 0u));
-    const float size_of = lane < a.groups && best > none
-                              ? fabsf((float)best) + (second > none ? fabsf((float)second) : 0.f)
-                              : 0.f;
-    const float mag = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(size_of)));
-    // A group without an expert (-inf) is not in doubt.
-    close = hi > -INFINITY &&
-            (a.bias ? too_close_biased(lo, hi, mag) : too_close_unbiased(lo, hi));
-  }
-  return close;
+  if (sizeof(S) != 4) return false;
+  const float magnitude = !counts || !(best > none) ? 0.f
+                          : fabsf((float)best) + (second > none ? fabsf((float)second) : 0.f);
+  return groups_close(a.bias != nullptr, counts, in, (float)score, magnitude);
 }
 
 // The chosen experts of a row, largest first, and their keys; one place more
@@ -474,15 +486,21 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __res
     total = row_sum<LANES>(total);
   }
   const float scale_of = rcp_fast(total);
-  float c[NV];
+  float c[NV], bias[NV];
   uint32_t key[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) bias[v] = 0.f;
+  if (a.bias) {
+    if (a.bias_runs) load_run<float, NV, true>(a.bias, i0, a.E, 0.f, bias);
+    else load_run<float, NV, false>(a.bias, i0, a.E, 0.f, bias);
+  }
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     c[v] = xv[v];
     if (scores) {
       const float s = a.sigmoid ? rcp_fast(1.f + ex2_fast(-kLog2e * xv[v]))
                                 : ex2_fast(kLog2e * (xv[v] - top)) * scale_of;
-      c[v] = a.bias && i0 + v < a.E ? fmaxf(s + a.bias[i0 + v], -INFINITY) : s;
+      c[v] = fmaxf(s + bias[v], -INFINITY);
       if (xv[v] == -INFINITY) c[v] = -INFINITY;
     }
     key[v] = key_of(a.bias ? c[v] : xv[v]);
@@ -689,9 +707,14 @@ bool runs_ok(const void* p, int64_t ld, int E, int NV) {
 }
 
 template <typename T, int LANES, int NV, bool GROUPED>
-int route_launch(const T* x, const RouteArgs& a, cudaStream_t st) {
+int route_launch(const T* x, const RouteArgs& given, cudaStream_t st) {
+  RouteArgs a = given;
   const int rows = ROUTE_THREADS / LANES;
   const unsigned grid = (unsigned)(((int64_t)a.T + rows - 1) / rows);
+  a.group_size = a.E / a.groups;
+  const int span = a.group_size / NV;
+  a.group_lanes = a.group_size % NV == 0 && (span & (span - 1)) == 0 ? span : 0;
+  a.bias_runs = a.E % NV == 0 && aligned16(a.bias);
   auto k = runs_ok<T>(x, a.ldx, a.E, NV) ? moe_route_kernel<T, LANES, NV, true, GROUPED>
                                          : moe_route_kernel<T, LANES, NV, false, GROUPED>;
   return launch_overlapped("moe_route_kernel", k, dim3(grid), ROUTE_THREADS, 0, 0, st, x, a);
@@ -770,7 +793,7 @@ extern "C" int ctb_moe_route(int32_t dtype, const void* logits, const float* bia
   if (!logits || !weights || !ids) return set_error(CTB_ERR_ARG, "moe_route: NULL pointer");
   DeviceProps pr;
   if (int rc = current_props(&pr)) return rc;
-  RouteArgs a;
+  RouteArgs a = {};
   a.bias = bias;
   a.weights = weights;
   a.ids = ids;
