@@ -147,6 +147,13 @@ __device__ __forceinline__ f2 normal_tail(f2 a, f2* density) {
   return mul2(mul2(p, t), e);
 }
 
+// |z|, at most 30, where Q has long been 0 (an infinity would make 0 * inf of
+// it); NaN stays NaN.
+__device__ __forceinline__ float tail_arg(float z) {
+  const float a = fabsf(z);
+  return a > 30.f ? 30.f : a;
+}
+
 // Both elements of a pair through the activation.
 template <int ACT>
 __device__ __forceinline__ void activate2(float& a, float& b) {
@@ -157,9 +164,10 @@ __device__ __forceinline__ void activate2(float& a, float& b) {
     const f2 z = mk2(a, b);
     un2(mul2(z, logistic_ex2(mul2(z, all2(-kLog2e)))), a, b);
   } else if (ACT == CTB_ACT_GELU) {  // z Phi(z) = max(z, 0) - |z| Q(|z|)
+    const float ta = tail_arg(a), tb = tail_arg(b);
     f2 e;
-    const f2 q = normal_tail(mk2(fabsf(a), fabsf(b)), &e);
-    un2(fma2(mk2(-fabsf(a), -fabsf(b)), q, mk2(fmaxf(a, 0.f), fmaxf(b, 0.f))), a, b);
+    const f2 q = normal_tail(mk2(ta, tb), &e);
+    un2(fma2(mk2(-ta, -tb), q, mk2(fmaxf(a, 0.f), fmaxf(b, 0.f))), a, b);
   } else if (ACT == CTB_ACT_GELU_TANH) {  // 0.5 (1 + tanh(u)) is the logistic function of 2 u
     const f2 z = mk2(a, b);
     const f2 u = mul2(z, fma2(mul2(z, z), all2(-kLog2e * kGeluScale * kGeluCube),
@@ -178,9 +186,10 @@ __device__ __forceinline__ void slope2(float& a, float& b) {
     const f2 s = logistic_ex2(mul2(z, all2(-kLog2e)));
     un2(mul2(s, fma2(z, fma2(s, all2(-1.f), all2(1.f)), all2(1.f))), a, b);
   } else if (ACT == CTB_ACT_GELU) {  // Phi(z) + z phi(z)
+    const float ta = tail_arg(a), tb = tail_arg(b);
     f2 e;
-    const f2 q = normal_tail(mk2(fabsf(a), fabsf(b)), &e);
-    const f2 d = mul2(mul2(mk2(a, b), all2(kInvSqrt2Pi)), e);
+    const f2 q = normal_tail(mk2(ta, tb), &e);
+    const f2 d = mul2(mul2(mk2(copysignf(ta, a), copysignf(tb, b)), all2(kInvSqrt2Pi)), e);
     float qa, qb;
     un2(q, qa, qb);
     un2(add2(d, mk2(a > 0.f ? 1.f - qa : qa, b > 0.f ? 1.f - qb : qb)), a, b);

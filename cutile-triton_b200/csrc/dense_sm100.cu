@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
   } else {
     uint32_t v[16];
     tmem_ld_32x32b_x16(tmem + lane_base, v);
-    tmem_ld_wait();
+    tmem_ld_wait_regs(v);
 #pragma unroll
     for (int j = 0; j < 16; ++j) partial[j * SP_COLS + threadIdx.x] = __uint_as_float(v[j]);
   }

@@ -189,6 +189,28 @@ def test_activation_extremes(dev):
         assert np.all(np.abs(C - ref) <= 2.0 ** -11 * np.abs(ref) + 2e-6 * (np.abs(f64(x)) + 1)[:, None] * (np.abs(ref) < 1e-3) + 2.0 ** -24)
 
 
+@pytest.mark.parametrize("N", [16, 300])
+def test_non_finite_values_through_the_activations(dev, N):
+    """NaN stays NaN; +inf is +inf; and a gradient of 0 at an infinite value
+    before the activation stays 0 under relu and gelu."""
+    A = torch.zeros(16, 16, dtype=torch.bfloat16, device=dev)
+    A[0, 0] = 1
+    B = torch.zeros(N, 16, dtype=torch.bfloat16, device=dev)
+    B[:3, 0] = torch.tensor([float("nan"), float("inf"), -float("inf")], device=dev)
+    for act in ACTS:
+        C = ops.dense(A, B, act=act)[:, 0]
+        assert bool(C[0].isnan()) and C[1].item() == float("inf")
+        assert C[2].item() == (-float("inf") if act == "none" else 0.0) or act in ("silu", "gelu_tanh")
+        assert bool((C[3:] == 0).all())
+    Z = torch.full((N, 16), float("inf"), dtype=torch.bfloat16, device=dev)
+    Z[::2] = -float("inf")
+    for act in ("relu", "gelu"):
+        dC = torch.zeros_like(Z)
+        dC[0, 0], dC[1, 1] = 2, 3  # slopes 0 at -inf, 1 at +inf
+        db = ops.dense_bwd(dC, A, torch.zeros_like(B), act=act, preact=Z)[2]
+        assert db.tolist() == [0.0, 3.0] + [0.0] * 14
+
+
 def test_strides_alignment_and_guards(dev):
     N, M, K = 40, 144, 80
     A, B, bias, R = inputs(dev, "f16", N, M, K, 5)
