@@ -93,7 +93,8 @@ def exact64(A, B, bias, act, R):
 @pytest.mark.parametrize("N,M,K,act", [(1, 4096, 4096, "silu"), (7, 14336, 1024, "gelu"),
                                        (96, 2048, 8192, "relu"), (1000, 2056, 520, "gelu"),
                                        (2049, 2304, 200, "silu"), (4096, 2560, 1024, "none"),
-                                       (2304, 4099, 333, "relu")])
+                                       (2304, 4099, 333, "relu"), (40000, 48, 64, "relu"),
+                                       (30000, 330, 40, "gelu"), (60001, 8, 128, "silu")])
 def test_dense_large(dev, dt, N, M, K, act):
     A, B, bias, R = inputs(dev, dt, N, M, K, 7)
     Z = torch.empty((N, M), dtype=DT[dt], device=dev)
@@ -166,7 +167,8 @@ def test_dense_gradients_of_each_activation(dev, dt, act):
 
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 @pytest.mark.parametrize("N,M,K,act", [(2049, 2304, 520, "silu"), (4096, 2560, 2048, "relu"),
-                                       (1000, 2307, 1003, "none"), (8, 4096, 4096, "silu")])
+                                       (1000, 2307, 1003, "none"), (8, 4096, 4096, "silu"),
+                                       (50000, 72, 56, "silu")])
 def test_dense_gradients_large(dev, dt, N, M, K, act):
     A, B, _, Z = inputs(dev, dt, N, M, K, 11)
     dC = torch.randn(N, M, generator=torch.Generator().manual_seed(4)).to(DT[dt]).to(dev)
