@@ -7,8 +7,8 @@
 // not of 128: the weight is then streamed once at memory speed, split over k so
 // that every SM has its share. Each CTA keeps its partial tile in its own
 // shared memory (Float32); the CTAs of a cluster then read one another's
-// partials over distributed shared memory (tiles of 16 rows: send them to the
-// row's owner) and add them in rank order, each finishing (bias, activation,
+// partials over distributed shared memory (tiles of up to 32 rows: send them to
+// the row's owner) and add them in rank order, each finishing (bias, activation,
 // residual, rounding) its share of the tile. No workspace, no atomics, the same
 // result every time.
 //
@@ -123,12 +123,12 @@ constexpr int SP_THREADS = 128;
 constexpr int SP_Q_BYTES = SP_COLS * BK * 2;
 // Stages for about 96 KB, so that two CTAs share an SM: one's epilogue runs
 // under the other's loads.
-__host__ __device__ constexpr int sp_stages(int BN) { return BN <= 32 ? 5 : BN == 64 ? 4 : 3; }
+__host__ __device__ constexpr int sp_stages(int BN) { return BN == 16 ? 5 : BN <= 64 ? 4 : 3; }
 __host__ __device__ constexpr int sp_stage_bytes(int BN) { return SP_Q_BYTES + BN * BK * 2; }
-// Tiles of 16 rows: room for the partial sums that the cluster's CTAs send (at
+// Tiles of up to 32 rows: room for the partial sums that the cluster's CTAs send (at
 // most BN + 7 rows, when BN rows are split over up to 8 owners).
 __host__ __device__ constexpr int sp_inbox_bytes(int BN) {
-  return BN == 16 ? (BN + 7) * SP_COLS * 4 : 0;
+  return BN <= 32 ? (BN + 7) * SP_COLS * 4 : 0;
 }
 constexpr int sp_smem(int BN) {
   return sp_stages(BN) * sp_stage_bytes(BN) + sp_inbox_bytes(BN) + 1024 + 256;
@@ -193,6 +193,13 @@ __device__ __forceinline__ void wait_received(uint64_t* bar, volatile int* abort
   }
 }
 
+__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&v)[32]) {
+  sm100::tmem_ld_32x32b_x32(addr, v);
+}
+__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&v)[16]) {
+  sm100::tmem_ld_32x32b_x16(addr, v);
+}
+
 // A producer that gave up waits (for at most a second each) until the loads it
 // has issued have landed, so that none outlives the CTA.
 __device__ __noinline__ void drain_loads(uint64_t* full, int64_t issued, int stages) {
@@ -234,12 +241,12 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
   const int kb0 = (int)((int64_t)a.num_kb * rank / S);
   const int kb1 = (int)((int64_t)a.num_kb * (rank + 1) / S);
   const int live_rows = (int)min((int64_t)BN, a.e.rows - r0);
-  // Tiles of 16 rows (a few tokens) are finished by owners: CTA r of the cluster
+  // Tiles of up to 32 rows (a few tokens) are finished by owners: CTA r of the cluster
   // owns `each` rows from r * each on, and the others send it their partial sums
   // of those, counted on its barrier. That is one way over distributed shared
   // memory instead of a barrier, a read and a closing barrier (1 x 4096 x 4096:
   // 0.25 + 0.6 us instead of 0.85 + 0.25 + 0.8).
-  const bool send = BN == 16 && S > 1;
+  const bool send = BN <= 32 && S > 1;
   const int each = (live_rows + (int)S - 1) / (int)S;
   const int owned = max(0, min(each, live_rows - (int)rank * each));
 
@@ -341,39 +348,28 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
   __syncwarp();
   tc_fence_after();
   const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-  if (BN >= 32) {
+  if (send) cluster_wait();  // every CTA's inbox is ready
+  uint32_t owner = 0;
+  int k = 0;  // the next row is row k of the owner's
+  constexpr int AT_ONCE = BN < 32 ? BN : 32;
 #pragma unroll 1
-    for (int r = 0; r < BN; r += 32) {
-      uint32_t v[32];
-      tmem_ld_32x32b_x32(tmem + lane_base + r, v);
-      tmem_ld_wait_regs(v);
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        partial[(r + j) * SP_COLS + threadIdx.x] = __uint_as_float(v[j]);
-    }
-  } else {
-    uint32_t v[16];
-    tmem_ld_32x32b_x16(tmem + lane_base, v);
+  for (int r = 0; r < BN; r += AT_ONCE) {
+    uint32_t v[AT_ONCE];
+    tmem_ld_rows(tmem + lane_base + r, v);
     tmem_ld_wait_regs(v);
-    if (send) {
-      cluster_wait();  // every CTA's inbox is ready
-      uint32_t owner = 0;
-      int k = 0;  // row j is row k of the owner's
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (j < live_rows) {
-          const uint32_t to = smem_u32(inbox + ((int)rank * min(each, live_rows - (int)owner * each) +
-                                                k) * SP_COLS + threadIdx.x);
-          st_async_cluster(mapa_shared(to, owner), v[j], mapa_shared(smem_u32(received), owner));
-          if (++k == each) {
-            k = 0;
-            ++owner;
-          }
+    for (int j = 0; j < AT_ONCE; ++j) {
+      if (!send) {
+        partial[(r + j) * SP_COLS + threadIdx.x] = __uint_as_float(v[j]);
+      } else if (r + j < live_rows) {
+        const int row = (int)rank * min(each, live_rows - (int)owner * each) + k;
+        st_async_cluster(mapa_shared(smem_u32(inbox + row * SP_COLS + threadIdx.x), owner), v[j],
+                         mapa_shared(smem_u32(received), owner));
+        if (++k == each) {
+          k = 0;
+          ++owner;
         }
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) partial[j * SP_COLS + threadIdx.x] = __uint_as_float(v[j]);
     }
   }
   tc_fence_before();
@@ -906,10 +902,10 @@ static bool rows16(const void* p, int64_t ld, int rows) {
 // A model of the two kernels' times in microseconds. Its numbers make the choice
 // by it the fastest one measured as nearly as possible over 1658 runs (150
 // products of 1 to 6000 rows, 256 to 14336 columns, 300 to 14336 k, each with
-// every tile and split): it takes 1.5% longer than the best, 18% at worst. A split
-// CTA takes its k-blocks at 80 GB/s, alone or beside another on its SM; 256 CTAs
+// every tile and split): it takes 1.2% longer than the best, 20% at worst. A split
+// CTA takes its k-blocks at 79 GB/s, alone or beside another on its SM; 256 CTAs
 // in clusters are sure to be resident at once, 296 single ones; more row tiles
-// read the weight again from L2. A pair takes 0.3 us a k-block and 3.2 us a tile.
+// read the weight again from L2. A pair takes 0.3 us a k-block and 3.1 us a tile.
 struct Plan {
   int BN, S;  // BN = 0: the pair kernel
 };
@@ -920,17 +916,16 @@ static double split_us(const Product& p, int BN, int S, int sms, double out_byte
   const int kb = (int)(((int64_t)p.depth + BK - 1) / BK), per = (kb + S - 1) / S;
   const double waves = std::ceil(ctas / (2 * sms));
   const double both = ctas > sms ? 2 : 1;
-  const double load = waves * per * sp_stage_bytes(BN) / 79.7e3;
-  const double moved = std::pow(tiles_r, 0.84) * 2.0 * p.cols * p.depth + 2.0 * p.rows * p.depth +
+  const double load = waves * per * sp_stage_bytes(BN) / 79e3;
+  const double moved = std::pow(tiles_r, 0.486) * 2.0 * p.cols * p.depth + 2.0 * p.rows * p.depth +
                        out_bytes;
-  return 2.25 + std::max(load, moved / 14.5e6) + waves * both * BN * 0.032 + (S > 1 ? 0.28 : 0) +
-         0.33 * S;
+  return 2.33 + std::max(load, moved / 9.66e6) + waves * both * BN * 0.032 + (S > 1 ? 0.22 : 0) +
+         0.21 * S;
 }
-static double pair_us(const Product& p, int pairs, double out_bytes) {
+static double pair_us(const Product& p, int pairs) {
   const double tiles = (double)(((int64_t)p.rows + 255) / 256 * (((int64_t)p.cols + 255) / 256));
   const int kb = (int)(((int64_t)p.depth + BK - 1) / BK);
-  const double moved = 2.0 * p.cols * p.depth + 2.0 * p.rows * p.depth + out_bytes;
-  return 3.6 + std::max(std::ceil(tiles / pairs) * (3.2 + 0.304 * kb), moved / 4.43e6);
+  return 3.7 + std::ceil(tiles / pairs) * (3.06 + 0.297 * kb);
 }
 
 // CTB_DENSE_PAIR=0 never takes the pair kernel, =1 whenever a pair can be resident.
@@ -945,7 +940,7 @@ static int pair_mode() {
 static Plan choose_plan(const Product& p, int sms, int pairs) {
   const double out_bytes = (1 + (p.Z ? 1 : 0) + (p.R ? 1 : 0)) * 2.0 * p.rows * p.cols;
   Plan best = {0, 1};
-  double us = pairs > 0 ? pair_us(p, pairs, out_bytes) : 1e30;
+  double us = pairs > 0 ? pair_us(p, pairs) : 1e30;
   const int mode = pair_mode();
   if (mode == 1 && pairs > 0) return best;
   if (mode == 0) us = 1e30;
