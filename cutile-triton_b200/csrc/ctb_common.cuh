@@ -74,7 +74,9 @@ __device__ __forceinline__ void flag_device_error(unsigned int bit) {
 // writes are visible. That hides a launch's latency and a kernel's set-up behind
 // the predecessor's tail. A kernel that allocates tensor memory lets the next
 // start only after the allocation: CTAs of the next one hold theirs while they
-// wait.
+// wait. What a predecessor may have written is read with ordinary loads, not
+// through the read-only path (no const __restrict__ parameters), whose data must
+// not change while the kernel runs.
 __device__ __forceinline__ void wait_for_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

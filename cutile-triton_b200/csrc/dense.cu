@@ -149,8 +149,8 @@ template <typename T> struct Columns<T, 1> {
 
 template <typename T, int W, int ACT>
 __global__ void __launch_bounds__(SLOPE_THREADS, 4)
-    slope_kernel(const T* __restrict__ dC, const T* __restrict__ Z, T* __restrict__ dZ,
-                 float* __restrict__ partial, int N, int M, int64_t lddc, int64_t ldz,
+    slope_kernel(const T* dC, const T* Z, T* dZ,
+                 float* partial, int N, int M, int64_t lddc, int64_t ldz,
                  int64_t lddz, int span) {
   let_next_start();
   wait_for_previous();
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(SLOPE_THREADS, 4)
 
 // Sums the spans: 32 columns a CTA, eight threads a column, joined in order.
 __global__ void __launch_bounds__(256)
-    fold_kernel(const float* __restrict__ partial, float* __restrict__ out, int M, int spans) {
+    fold_kernel(const float* partial, float* out, int M, int spans) {
   let_next_start();
   wait_for_previous();
   __shared__ float red[8][32];

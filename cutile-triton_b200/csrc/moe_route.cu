@@ -49,7 +49,7 @@ template <> struct Raw<16> { using type = uint4; };
 
 // NV neighbouring values of a row, as vectors of at most 16 bytes where VEC.
 template <typename T, int NV, bool VEC>
-__device__ __forceinline__ void load_run(const T* __restrict__ p, int i0, int E, float pad,
+__device__ __forceinline__ void load_run(const T* p, int i0, int E, float pad,
                                          float (&v)[NV]) {
   if (VEC) {
     constexpr int W = NV * (int)sizeof(T) < 16 ? NV : 16 / (int)sizeof(T);
@@ -75,7 +75,7 @@ __device__ __forceinline__ void load_run(const T* __restrict__ p, int i0, int E,
   }
 }
 template <typename T, int NV, bool VEC>
-__device__ __forceinline__ void store_run(T* __restrict__ p, int i0, int E, const float (&v)[NV]) {
+__device__ __forceinline__ void store_run(T* p, int i0, int E, const float (&v)[NV]) {
   if (VEC) {
     constexpr int W = NV * (int)sizeof(T) < 16 ? NV : 16 / (int)sizeof(T);
     using R = typename Raw<W * (int)sizeof(T)>::type;
@@ -415,7 +415,7 @@ __device__ __forceinline__ bool neighbours_close(const Chosen* row, int topk) {
 
 // The same row ranked in 64 bits.
 template <typename T, int LANES, int NV, bool GROUPED>
-__device__ __noinline__ void choose_exact(const RouteArgs& a, const T* __restrict__ x, int i0,
+__device__ __noinline__ void choose_exact(const RouteArgs& a, const T* x, int i0,
                                           bool in_range, Chosen* sel, double* row) {
   double c[NV];
   uint64_t key[NV];
@@ -449,7 +449,7 @@ __device__ __noinline__ void choose_exact(const RouteArgs& a, const T* __restric
 }
 
 template <typename T, int LANES, int NV, bool VEC, bool GROUPED>
-__global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* __restrict__ x,
+__global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* x,
                                                                   const RouteArgs a) {
   constexpr int ROWS = ROUTE_THREADS / LANES;
   constexpr int SLOTS = ROUTE_MAX_TOPK / LANES;  // places of a row per lane
@@ -587,7 +587,7 @@ struct RouteBwdArgs {
 
 template <typename T, int LANES, int NV, bool VEC>
 __global__ void __launch_bounds__(ROUTE_THREADS)
-    moe_route_bwd_kernel(const T* __restrict__ x, T* __restrict__ dx, const RouteBwdArgs a) {
+    moe_route_bwd_kernel(const T* x, T* dx, const RouteBwdArgs a) {
   constexpr int ROWS = ROUTE_THREADS / LANES;
   constexpr int SLOTS = ROUTE_MAX_TOPK / LANES;
   __shared__ int2 slot_all[ROWS][ROUTE_MAX_TOPK];  // (expert, gradient bits) of each place

@@ -150,3 +150,44 @@ def test_offsets_past_32_bits(dev):
     tail = C[N - 40:].double() @ A.double().t()
     assert rel(dB[N - 40:], tail) <= 2.0 ** -11 + 1e-4
     ops.check_device()
+
+
+@pytest.mark.parametrize("T,D,hidden", [(1, 128, 512), (40, 256, 1024), (600, 520, 2304)])
+def test_back_to_back_is_as_with_waits_between(dev, T, D, hidden):
+    """Kernels start under the tail of the one before. A chain that reads what
+    was just written, writes in place over what was just read and changes
+    its weights gives the same bits whether or not each call is waited for."""
+    E, topk = 8, 2
+    g = torch.Generator(device=dev).manual_seed(T)
+    r = lambda *s, k=1.0: (torch.randn(*s, generator=g, device=dev) * k).bfloat16()  # noqa: E731
+    x0, up0, down0 = r(T, D), r(D, hidden, k=D ** -0.5), r(hidden, D, k=hidden ** -0.5)
+    gate, bias = r(D, E, k=D ** -0.5), torch.randn(hidden, generator=g, device=dev)
+
+    def chain(wait):
+        x, up, down = x0.clone(), up0.clone(), down0.clone()
+        h, z = torch.empty(T, hidden, dtype=x.dtype, device=dev), torch.empty(T, hidden, dtype=x.dtype, device=dev)
+        y = torch.empty(T * topk, D, dtype=x.dtype, device=dev)
+        steps = []
+
+        def step(out):
+            steps.append(out)
+            if wait:
+                torch.cuda.synchronize()
+            return out
+
+        for _ in range(12):
+            step(ops.dense(up, x, bias=bias, act="gelu", out=h, preact=z))
+            step(ops.dense(down, h, residual=x, out=x))
+            w, i = step(ops.moe_route(ops.dense(gate, x), topk))
+            dy, _ = step(ops.moe_combine_bwd(x, None, topk, dy=y))
+            step(ops.moe_combine(dy, topk, w, i, E, out=x))
+            dx = step(ops.dense_bwd(h, up, x, act="gelu", preact=z))
+            step(ops.moe_combine(x, 1, residual=dx[1], out=x))
+            up.add_(dx[0], alpha=1e-3)  # another library's kernel in between
+            x.div_(x.float().norm() / (T * D) ** 0.5 + 1e-3)
+        torch.cuda.synchronize()
+        return [x, up, h, z, y, w, i]
+
+    for a, b in zip(chain(True), chain(False)):
+        assert torch.equal(a, b)
+    assert bool(torch.isfinite(chain(False)[0]).all())
