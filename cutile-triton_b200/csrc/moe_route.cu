@@ -146,12 +146,18 @@ __device__ __forceinline__ uint32_t row_max_key(uint32_t v) {
 }
 template <int LANES>
 __device__ __forceinline__ uint64_t row_max_key(uint64_t v) {
+  if constexpr (LANES == 32) {  // the high words' maximum, then the low words' among those
+    const uint32_t hi = __reduce_max_sync(FULL, (uint32_t)(v >> 32));
+    const uint32_t lo = __reduce_max_sync(FULL, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+    return (uint64_t)hi << 32 | lo;
+  } else {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor_sync(FULL, v, o);
-    v = w > v ? w : v;
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      const uint64_t w = __shfl_xor_sync(FULL, v, o);
+      v = w > v ? w : v;
+    }
+    return v;
   }
-  return v;
 }
 
 struct RouteArgs {
@@ -183,16 +189,17 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Whether two choice values hi >= lo are too close for 32 bits to order them.
 // 2^(d log2 e) carries at most 2.4e-7 (ex2.approx) + 2e-7 |d| (the roundings of
-// d, of log2 e and of their product) relative error; the row's sum (its terms'
-// errors weighted, 8 levels of additions) at most 2e-6, reciprocal and product
-// 2.4e-7.
-// With a bias, the scores of a pair (or of two groups) of one row err by at
-// most 4e-6 together (softmax: they add up to at most 1; sigmoid: under 6e-7
-// each), and each addition by 2^-24 of the magnitude `mag`. Without one the
-// error is relative, |ln hi| standing for |d|; sums so small that 32 bits lose
-// them are never certain.
-__device__ __forceinline__ bool too_close_biased(float hi, float lo, float mag) {
-  return !(hi - lo > 4e-6f + 5e-7f * mag);
+// d, of log2 e and of their product) relative error. Of a sigmoid that is s (1 -
+// s) times as much, at most 7e-8, and its sum and reciprocal add 1.8e-7: 2.5e-7
+// each, 6e-7 the two of a pair, 1.2e-6 the four of two groups. Of a softmax the
+// row's sum (its terms' errors weighted, 8 levels of additions) adds at most
+// 2e-6, reciprocal and product 2.4e-7; a row's scores add up to at most 1, so two
+// or four of them err by at most 4e-6 together. Each addition (of a bias, of a
+// group's two) adds 2^-24 of its result: 1e-7 of the magnitudes of a pair, 3e-7
+// of the largest group's. Without a bias the error is relative, |ln hi| standing
+// for |d|; sums so small that 32 bits lose them are never certain.
+__device__ __forceinline__ bool too_close(float hi, float lo, float error) {
+  return !(hi - lo > error);
 }
 __device__ __forceinline__ bool too_close_unbiased(float hi, float lo) {
   return !(hi > 1e-30f && hi - lo > 2.f * hi * (4e-6f + 2.5e-7f * fabsf(__logf(hi))));
@@ -200,14 +207,16 @@ __device__ __forceinline__ bool too_close_unbiased(float hi, float lo) {
 
 // Whether the order between the kept groups (`in`) and the others is too close
 // for 32 bits; each lane holds a group's score and the magnitude of its terms.
-__device__ __forceinline__ bool groups_close(bool biased, bool counts, bool in, float score,
+__device__ __forceinline__ bool groups_close(const RouteArgs& a, bool counts, bool in, float score,
                                              float magnitude) {
   const uint32_t k = key_of(score);
   const float lo = value_of(__reduce_min_sync(FULL, counts && in ? k : 0xffffffffu));
   const float hi = value_of(__reduce_max_sync(FULL, counts && !in ? k : kNone32));
   const float mag = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(magnitude)));
   // A group without an expert (-inf) is not in doubt.
-  return hi > -INFINITY && (biased ? too_close_biased(lo, hi, mag) : too_close_unbiased(lo, hi));
+  return hi > -INFINITY &&
+         (a.bias ? too_close(lo, hi, (a.sigmoid ? 1.2e-6f : 4e-6f) + 3e-7f * mag)
+                 : too_close_unbiased(lo, hi));
 }
 
 // Keys of the experts outside the best topk_groups groups become 0 (c is -inf
@@ -251,7 +260,7 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV]
     if (sizeof(S) != 4) return false;
     const float magnitude = !counts || !(best > none) ? 0.f
                             : fabsf((float)best) + (second > none ? fabsf((float)second) : 0.f);
-    return groups_close(a.bias != nullptr, counts, in, (float)score, magnitude);
+    return groups_close(a, counts, in, (float)score, magnitude);
   }
   // Through shared memory, a lane per group; one word in 32 is skipped so that
   // lanes that start a multiple of 32 apart use different banks.
@@ -288,7 +297,7 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV]
   if (sizeof(S) != 4) return false;
   const float magnitude = !counts || !(best > none) ? 0.f
                           : fabsf((float)best) + (second > none ? fabsf((float)second) : 0.f);
-  return groups_close(a.bias != nullptr, counts, in, (float)score, magnitude);
+  return groups_close(a, counts, in, (float)score, magnitude);
 }
 
 // The chosen experts of a row, largest first, and their keys; one place more
@@ -401,19 +410,20 @@ __device__ __forceinline__ void choose(K (&key)[NV], Chosen* row, uint64_t* cand
 // Whether two neighbours in the order (the first one left out included) are
 // too close.
 template <int LANES>
-__device__ __forceinline__ bool neighbours_close(const Chosen* row, int topk) {
+__device__ __forceinline__ bool neighbours_close(const RouteArgs& a, const Chosen* row) {
   bool close = false;
-  for (int j = threadIdx.x % LANES; j < topk; j += LANES) {
+  for (int j = threadIdx.x % LANES; j < a.topk; j += LANES) {
     const uint32_t hi = row->key[j], lo = row->key[j + 1];
     if (lo) {
       const float x = value_of(hi), y = value_of(lo);
-      close |= too_close_biased(x, y, fabsf(x) + fabsf(y));
+      close |= too_close(x, y, (a.sigmoid ? 6e-7f : 4e-6f) + 1e-7f * (fabsf(x) + fabsf(y)));
     }
   }
   return close;
 }
 
-// The same row ranked in 64 bits.
+// The same row ranked in 64 bits. The loops with an exponential stay rolled: the
+// code is rarely run, so its length (instruction misses) is most of its time.
 template <typename T, int LANES, int NV, bool GROUPED>
 __device__ __noinline__ void choose_exact(const RouteArgs& a, const T* x, int i0,
                                           bool in_range, Chosen* sel, double* row) {
@@ -432,14 +442,15 @@ __device__ __noinline__ void choose_exact(const RouteArgs& a, const T* x, int i0
     for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(FULL, top, o));
     if (top == -INFINITY) top = 0.0;
     total = 0.0;
-#pragma unroll
+#pragma unroll 1
     for (int v = 0; v < NV; ++v) total += exp(c[v] - top);
     total = row_sum<LANES>(total);
   }
-#pragma unroll
+#pragma unroll 1
   for (int v = 0; v < NV; ++v) {
     const double xv = c[v];
-    const double s = a.sigmoid ? 1.0 / (1.0 + exp(-xv)) : exp(xv - top) / total;
+    const double e = exp(a.sigmoid ? -xv : xv - top);
+    const double s = (a.sigmoid ? 1.0 : e) / (a.sigmoid ? 1.0 + e : total);
     c[v] = a.bias && i0 + v < a.E ? s + (double)a.bias[i0 + v] : s;
     if (!(xv > -INFINITY && c[v] > -INFINITY)) c[v] = -INFINITY;
     key[v] = key_of(a.bias || !(c[v] > -INFINITY) ? c[v] : xv);
@@ -511,7 +522,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* x,
   const bool check = a.bias != nullptr;
   choose<uint32_t, LANES, NV>(key, sel, cand[LANES == 32 ? threadIdx.x / 32 : 0],
                               a.topk + (check ? 1 : 0));
-  if (check) close |= neighbours_close<LANES>(sel, a.topk);
+  if (check) close |= neighbours_close<LANES>(a, sel);
   if (__any_sync(FULL, close && in_range))
     choose_exact<T, LANES, NV, GROUPED>(a, xr, i0, in_range, sel, row);
 
