@@ -169,6 +169,7 @@ struct RouteArgs {
   int sigmoid, groups, topk_groups, group_top, renorm;
   int group_size;   // experts per group
   int group_lanes;  // lanes per group where that is a power of two of whole lanes, else 0
+  float pair_error; // of the scores of two experts of a row together
   bool bias_runs;   // the bias is made of whole runs of NV floats, 16-byte aligned
   float scale;
 };
@@ -305,6 +306,7 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, const S (&c)[NV]
 struct Chosen {
   int id[ROUTE_MAX_TOPK + 1];
   uint32_t key[ROUTE_MAX_TOPK + 1];  // of the 32-bit choice
+  int candidates;                    // how many the choice was made from; -1: all experts
 };
 
 // Fills row->id[0..rounds), -1 where no expert is left, and row->key for 32-bit keys.
@@ -314,11 +316,13 @@ struct Chosen {
 // for the best 8 of random scores); those candidates move to one lane each, and
 // a lane's rank among them is its place. 160 instructions for 8 of 256, against
 // 450 for choosing one after the other, which is left for rows with more than
-// 32 candidates, for narrower rows and for 64 bits. There a lane knows its two
+// 32 candidates, for narrower rows and for 64 bits. `slack` lowers the bound so
+// that whatever 64 bits could choose instead is a candidate too. There a lane knows its two
 // best, so that it looks through its registers again only when it has been
 // chosen from twice.
 template <typename K, int LANES, int NV>
-__device__ __forceinline__ void choose(K (&key)[NV], Chosen* row, uint64_t* cand, int rounds) {
+__device__ __forceinline__ void choose(K (&key)[NV], Chosen* row, uint64_t* cand, int rounds,
+                                       float slack) {
   const int lane = threadIdx.x & 31, sub = lane % LANES, base = lane - sub;
   if constexpr (LANES == 32 && sizeof(K) == 4) {
     uint32_t t = key[0], bound = 0;
@@ -330,6 +334,10 @@ __device__ __forceinline__ void choose(K (&key)[NV], Chosen* row, uint64_t* cand
       if (t == bound) t = 0;
     }
     bound = max(bound, kNone32 + 1);
+    if (slack > 0.f && bound > kNone32 + 1) {
+      const float b = value_of(bound);
+      if (b < INFINITY) bound = max(key_of(b - (slack + 2e-7f * fabsf(b))), kNone32 + 1);
+    }
     int total = 0, at[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -356,10 +364,14 @@ __device__ __forceinline__ void choose(K (&key)[NV], Chosen* row, uint64_t* cand
         row->id[place] = mine ? (int)~(uint32_t)mine : -1;
         row->key[place] = (uint32_t)(mine >> 32);
       }
-      if (rounds > 32 && lane == 0) row->key[32] = 0;
+      if (lane == 0) {
+        if (rounds > 32) row->key[32] = 0;
+        row->candidates = total;
+      }
       __syncwarp();
       return;
     }
+    if (lane == 0) row->candidates = -1;
   }
   K k1 = 0, k2 = 0;
   int v1 = 0, v2 = 0;
@@ -416,7 +428,7 @@ __device__ __forceinline__ bool neighbours_close(const RouteArgs& a, const Chose
     const uint32_t hi = row->key[j], lo = row->key[j + 1];
     if (lo) {
       const float x = value_of(hi), y = value_of(lo);
-      close |= too_close(x, y, (a.sigmoid ? 6e-7f : 4e-6f) + 1e-7f * (fabsf(x) + fabsf(y)));
+      close |= too_close(x, y, a.pair_error + 1e-7f * (fabsf(x) + fabsf(y)));
     }
   }
   return close;
@@ -456,7 +468,39 @@ __device__ __noinline__ void choose_exact(const RouteArgs& a, const T* x, int i0
     key[v] = key_of(a.bias || !(c[v] > -INFINITY) ? c[v] : xv);
   }
   if (GROUPED) keep_groups<double, NV>(a, c, key, row);
-  choose<uint64_t, LANES, NV>(key, sel, nullptr, a.topk);
+  choose<uint64_t, LANES, NV>(key, sel, nullptr, a.topk, 0.f);
+}
+
+// The candidates of a whole warp's row ranked again in 64 bits, one to a lane.
+template <typename T, int NV>
+__device__ __noinline__ void rank_exact(const RouteArgs& a, const T* x, int i0, float top,
+                                        Chosen* sel, uint64_t* cand) {
+  const int lane = threadIdx.x & 31, total = sel->candidates;
+  const int id = lane < total ? (int)~(uint32_t)cand[lane] : 0;
+  double sum = 1.0;
+  if (!a.sigmoid) {
+    sum = 0.0;
+#pragma unroll 1
+    for (int v = 0; v < NV; ++v) {
+      const double xv = i0 + v < a.E ? (double)to_float(x[i0 + v]) : -INFINITY;
+      sum += isnan(xv) ? 0.0 : exp(xv - (double)top);
+    }
+    sum = row_sum<32>(sum);
+  }
+  const double xv = (double)to_float(x[id]);
+  const double e = exp(a.sigmoid ? -xv : xv - (double)top);
+  const double s = (a.sigmoid ? 1.0 : e) / (a.sigmoid ? 1.0 + e : sum);
+  const uint64_t mine = key_of(s + (double)a.bias[id]);
+  __syncwarp();
+  cand[lane] = mine;
+  __syncwarp();
+  int place = 0;
+  for (int i = 0; i < total; ++i) {
+    const int other = __shfl_sync(FULL, id, i);
+    place += cand[i] > mine || (cand[i] == mine && other < id);
+  }
+  if (lane < total && place < a.topk) sel->id[place] = id;
+  __syncwarp();
 }
 
 template <typename T, int LANES, int NV, bool VEC, bool GROUPED>
@@ -521,10 +565,19 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* x,
   if (GROUPED) close = keep_groups<float, NV>(a, c, key, reinterpret_cast<float*>(row));
   const bool check = a.bias != nullptr;
   choose<uint32_t, LANES, NV>(key, sel, cand[LANES == 32 ? threadIdx.x / 32 : 0],
-                              a.topk + (check ? 1 : 0));
-  if (check) close |= neighbours_close<LANES>(a, sel);
-  if (__any_sync(FULL, close && in_range))
+                              a.topk + (check ? 1 : 0), check ? a.pair_error : 0.f);
+  const bool order = check && neighbours_close<LANES>(a, sel);
+  if (LANES == 32) {
+    if (in_range && (__any_sync(FULL, close) || __any_sync(FULL, order))) {
+      // Only the order of the candidates is in doubt, unless it is the groups'.
+      if (__any_sync(FULL, close) || sel->candidates < 0)
+        choose_exact<T, LANES, NV, GROUPED>(a, xr, i0, in_range, sel, row);
+      else
+        rank_exact<T, NV>(a, xr, i0, top, sel, cand[LANES == 32 ? threadIdx.x / 32 : 0]);
+    }
+  } else if (__any_sync(FULL, order && in_range)) {
     choose_exact<T, LANES, NV, GROUPED>(a, xr, i0, in_range, sel, row);
+  }
 
   // Weights: place j belongs to lane j % LANES of its row.
   float xs[SLOTS], w[SLOTS];
@@ -726,6 +779,7 @@ int route_launch(const T* x, const RouteArgs& given, cudaStream_t st) {
   const int span = a.group_size / NV;
   a.group_lanes = a.group_size % NV == 0 && (span & (span - 1)) == 0 ? span : 0;
   a.bias_runs = a.E % NV == 0 && aligned16(a.bias);
+  a.pair_error = a.sigmoid ? 6e-7f : 4e-6f;
   auto k = runs_ok<T>(x, a.ldx, a.E, NV) ? moe_route_kernel<T, LANES, NV, true, GROUPED>
                                          : moe_route_kernel<T, LANES, NV, false, GROUPED>;
   return launch_overlapped("moe_route_kernel", k, dim3(grid), ROUTE_THREADS, 0, 0, st, x, a);

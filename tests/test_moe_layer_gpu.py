@@ -126,6 +126,17 @@ def test_route_ties_and_values_closer_than_float32(dev):
         for score in ("sigmoid", "softmax"):
             check_route(dev, x.to(dev), min(8, E), score=score, bias=bias.float(), groups=groups,
                         topk_groups=keep)
+    # A whole warp's row: a few that tie in Float32 (100 steps), more of them than
+    # lanes (3 steps); and groups that are certain while the order within is not.
+    for E, groups, keep, steps in ((256, 1, 1, 100), (256, 1, 1, 3), (200, 1, 1, 60),
+                                   (256, 8, 2, 12), (130, 5, 2, 20)):
+        x = torch.randn(300, E, generator=g) * 1e-6
+        x[::7, ::3] = float("-inf")
+        bias = 1000.0 + torch.randint(0, steps, (E,), generator=g) * 6.1e-5
+        bias += torch.arange(E) // (E // groups) * 10.0
+        for score in ("sigmoid", "softmax"):
+            check_route(dev, x.to(dev), 8, score=score, bias=bias.float(), groups=groups,
+                        topk_groups=keep, renorm=False)
     # group sums far below 1: softmax of a row with one dominant expert
     x = torch.randn(300, 64, generator=g) * 1e-5 - 60
     x[:, 0] = 30
