@@ -14,13 +14,18 @@
 // The choice is the one of exact arithmetic. Without a bias the experts of a
 // row rank as their logits do, which needs no arithmetic. With a bias, and
 // between groups, c is computed in 32 bits first; where two values that decide
-// the order are closer than those 32 bits tell apart (a few rows in a
-// thousand), the row is ranked again in 64 bits.
+// the order are closer than those 32 bits tell apart (about one row in a
+// thousand), the candidates, or where groups are in doubt the whole row, are
+// ranked again in 64 bits.
 //
 // A row belongs to LANES lanes of a warp, NV neighbouring experts to a lane, so
 // that a tie goes to the first lane and the first register. Each choice is one
 // maximum over the lanes and a rescan of the winner's NV registers. Rows of up
 // to 64 experts take 8 lanes (four rows per warp).
+//
+// Bound by instruction issue (IPC 2.5 to 3.2), not by HBM: 65536 x 256 f32 takes 39
+// us without a bias and 62 with bias and groups (800 instructions a row) against
+// 10 at the copy rate; 16384 rows 16.5 us.
 #include "ctb_common.cuh"
 
 #include <algorithm>
@@ -638,7 +643,8 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* x,
 //   sigmoid         dx = g s (1 - s)                     chosen experts only
 //   sigmoid, renorm dx = p (1 - s) * (g - sum(g p))      chosen experts only
 // One pass: the row (plain softmax) or the chosen logits are read, the whole
-// row of dx is written once.
+// row of dx is written once. 65536 x 256 f32 plain softmax: 38 us, 20 at the copy
+// rate; 16384 x 64: 4.8 us with its launch.
 // -----------------------------------------------------------------------------
 struct RouteBwdArgs {
   const float* dweights;
