@@ -373,7 +373,8 @@ extern "C" int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const 
     return set_error(CTB_ERR_LAYOUT, "dense: leading dimension smaller than the column length");
   if (M == 0 || N == 0) return CTB_OK;
   if (!C || (K > 0 && (!A || !B))) return set_error(CTB_ERR_ARG, "dense: NULL pointer");
-  if (Z && (Z == C || Z == R)) return set_error(CTB_ERR_ARG, "dense: Z must be a matrix of its own");
+  if (C == A || C == B || (Z && (Z == C || Z == R || Z == A || Z == B)))
+    return set_error(CTB_ERR_ARG, "dense: C and Z must be matrices of their own (C may be R)");
   const int64_t need = ctb_dense_fwd_workspace_bytes(A, B, M, N, K, lda, ldb);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return set_error(CTB_ERR_ARG, "dense: the workspace needs " + std::to_string(need) +
@@ -420,6 +421,11 @@ extern "C" int ctb_dense_bwd(int32_t dtype, const void* dC, const void* A, const
   const bool some = M > 0 && N > 0;
   if ((some && (!dC || (slope && !Z))) || (some && K > 0 && ((dB && !A) || (dA && !B))))
     return set_error(CTB_ERR_ARG, "dense_bwd: NULL pointer");
+  for (const void* out : {(const void*)dA, (const void*)dB, (const void*)dbias})
+    if (out && (out == dC || out == A || out == B || out == Z))
+      return set_error(CTB_ERR_ARG, "dense_bwd: gradients must be matrices of their own");
+  if (dA && dA == dB)
+    return set_error(CTB_ERR_ARG, "dense_bwd: gradients must be matrices of their own");
   const int64_t need = ctb_dense_bwd_workspace_bytes(dC, A, B, M, N, K, lddc, lda, ldb, act,
                                                      dbias != nullptr);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))

@@ -291,6 +291,8 @@ extern "C" int ctb_moe_combine(int32_t dtype, const void* y, const float* weight
     return set_error(CTB_ERR_LAYOUT, "moe_combine: row stride smaller than the row");
   if (T == 0 || N == 0) return CTB_OK;
   if (!y || !out) return set_error(CTB_ERR_ARG, "moe_combine: NULL pointer");
+  if (out == y && topk > 1)
+    return set_error(CTB_ERR_ARG, "moe_combine: out over y needs one slot per token");
   DeviceProps pr;
   if (int rc = current_props(&pr)) return rc;
   auto st = static_cast<cudaStream_t>(stream);
@@ -323,6 +325,8 @@ extern "C" int ctb_moe_combine_bwd(int32_t dtype, const void* dout, const void* 
   if (T == 0) return CTB_OK;
   if ((N > 0 && (!dout || !dy)) || (weights && (!dweights || (N > 0 && !y))))
     return set_error(CTB_ERR_ARG, "moe_combine_bwd: NULL pointer");
+  if (dy == dout && N > 0 && topk > 1)
+    return set_error(CTB_ERR_ARG, "moe_combine_bwd: dy over dout needs one slot per token");
   DeviceProps pr;
   if (int rc = current_props(&pr)) return rc;
   auto st = static_cast<cudaStream_t>(stream);

@@ -382,7 +382,8 @@ int ctb_moe_route_bwd(int32_t dtype, const float* dweights, const void* logits,
  * summed in Float32 in the order of j, rounded once. y: T * topk rows of N
  * contiguous elements, dtype F16 or BF16, row stride ldy; weights: T x topk
  * floats or NULL (all 1: ctb_moe_gemm_f16 may have applied them); residual:
- * row stride ldr, or NULL; out: row stride ldo, may be the residual itself.
+ * row stride ldr, or NULL; out: row stride ldo, may be the residual itself
+ * (and y itself where topk is 1).
  * ids: T x topk or NULL; a slot whose id is outside [0, E) was given to no
  * expert: its row of y is not read and its weight not used. */
 int ctb_moe_combine(int32_t dtype, const void* y, const float* weights, const int32_t* ids,

@@ -74,6 +74,26 @@ def test_dense_bwd_refusals(kw, code):
         a["wsb"], None) == code
 
 
+@pytest.mark.parametrize("same", [("C", "A"), ("C", "B"), ("Z", "A"), ("Z", "B"), ("Z", "C"), ("Z", "R")])
+def test_dense_refuses_outputs_over_inputs(same):
+    p = {k: NP + 4096 * i for i, k in enumerate("ABCZR")}
+    p[same[0]] = p[same[1]]
+    assert _lib.load().ctb_dense_fwd(_lib.CTB_F16, p["A"], p["B"], None, 0, p["R"], p["Z"], p["C"], 16,
+                                     4, 32, 16, 32, 16, 16, 16, 0, None, 0, None) == -1
+    assert b"of their own" in _lib.load().ctb_last_error()
+
+
+@pytest.mark.parametrize("same", [("dA", "A"), ("dA", "B"), ("dA", "dC"), ("dB", "B"), ("dB", "dC"),
+                                  ("dB", "Z"), ("dA", "dB"), ("db", "dC")])
+def test_dense_bwd_refuses_outputs_over_inputs(same):
+    p = {k: NP + 4096 * i for i, k in enumerate(("dC", "A", "B", "Z", "dA", "dB", "db"))}
+    p[same[0]] = p[same[1]]
+    assert _lib.load().ctb_dense_bwd(_lib.CTB_F16, p["dC"], p["A"], p["B"], p["Z"], p["dA"], p["dB"],
+                                     p["db"], 16, 4, 32, 16, 16, 32, 16, 16, 32, 4, NP, 1 << 30,
+                                     None) == -1
+    assert b"of their own" in _lib.load().ctb_last_error()
+
+
 def test_workspace_sizes():
     L = _lib.load()
     assert L.ctb_dense_fwd_workspace_bytes(NP, NP, 4096, 7, 512, 4096, 512) == 0

@@ -108,6 +108,7 @@ def test_route_bwd_refusals(kw, code):
     (dict(dtype=_lib.CTB_F32), -2), (dict(T=-1), -3), (dict(N=-1), -3), (dict(topk=0), -3),
     (dict(T=1 << 30, topk=4), -3), (dict(ids=NP, E=0), -3), (dict(ldy=15), -4),
     (dict(ldo=15), -4), (dict(res=NP, ldr=15), -4), (dict(y=None), -1), (dict(out=None), -1),
+    (dict(out=NP + 4096, y=NP + 4096), -1),
     (dict(T=0, y=None), 0), (dict(N=0, ldy=0, ldo=0, y=None), 0),
 ])
 def test_combine_refusals(kw, code):
@@ -122,7 +123,7 @@ def test_combine_refusals(kw, code):
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=_lib.CTB_F32), -2), (dict(T=-1), -3), (dict(topk=-2), -3), (dict(lddo=15), -4),
     (dict(ldy=15), -4), (dict(lddy=15), -4), (dict(d=None), -1), (dict(y=None), -1),
-    (dict(dy=None), -1), (dict(dw=None), -1), (dict(T=0, d=None), 0), (dict(ids=NP, E=-1), -3),
+    (dict(dy=None), -1), (dict(dw=None), -1), (dict(dy=NP), -1), (dict(T=0, d=None), 0), (dict(ids=NP, E=-1), -3),
 ])
 def test_combine_bwd_refusals(kw, code):
     a = dict(dtype=_lib.CTB_BF16, d=NP, y=NP, w=NP, ids=None, dy=NP, dw=NP, T=4, topk=2, N=16, E=4,
