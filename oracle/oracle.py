@@ -259,7 +259,8 @@ def activation(z, act):
     if act == "relu":
         return np.maximum(z, 0), (z > 0).astype(np.float64)
     if act == "silu":
-        s = 1 / (1 + np.exp(-z))
+        with np.errstate(over="ignore"):
+            s = 1 / (1 + np.exp(-z))
         return z * s, s * (1 + z * (1 - s))
     if act == "gelu":
         erfc = np.vectorize(math.erfc, otypes=[np.float64])
