@@ -177,30 +177,32 @@ __global__ void __launch_bounds__(COMBINE_THREADS)
   const T* d = a.dout + s / a.topk * a.lddo;
   const T* y = a.y + (a.weights ? s * a.ldy : 0);
   T* dy = a.dy + s * a.lddy;
+  // Unsigned columns: the step past the end of the longest row (2^31 - 1) does not wrap.
+  const uint32_t N = (uint32_t)a.N, first = (uint32_t)lane * W;
   float dot = 0.f;
   if (!used) {
     float z[W];
 #pragma unroll
     for (int e = 0; e < W; ++e) z[e] = 0.f;
-    for (int c = lane * W; c < a.N; c += 32 * W) Run<T, W>::put(dy + c, z);
+    for (uint32_t c = first; c < N; c += 32 * W) Run<T, W>::put(dy + c, z);
   } else {
     // FLIGHT runs of both rows are asked for before the first is used (the
     // stores between them could alias, so the compiler would not).
     constexpr int FLIGHT = 4;
-    for (int c0 = lane * W; c0 < a.N; c0 += FLIGHT * 32 * W) {
+    for (uint32_t c0 = first; c0 < N; c0 += FLIGHT * 32 * W) {
       Run<T, W> rd[FLIGHT], ry[FLIGHT];
 #pragma unroll
       for (int j = 0; j < FLIGHT; ++j) {
-        const int c = c0 + j * 32 * W;
-        if (c < a.N) {
+        const uint32_t c = c0 + j * 32 * W;
+        if (c < N) {
           rd[j].load(d + c);
           if (a.weights) ry[j].load_once(y + c);
         }
       }
 #pragma unroll
       for (int j = 0; j < FLIGHT; ++j) {
-        const int c = c0 + j * 32 * W;
-        if (c < a.N) {
+        const uint32_t c = c0 + j * 32 * W;
+        if (c < N) {
           float fd[W], fy[W];
           rd[j].get(fd);
           if (a.weights) {
