@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack first, const Pack 
   let_next_start();
   wait_for_previous();
   const Pack& k = blockIdx.y ? second : first;
-  const int runs = (k.len + 7) / 8;
+  const int runs = (int)(((int64_t)k.len + 7) / 8);  // a length may be 2^31 - 1
   const int64_t total = k.lines * runs;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * 256) {

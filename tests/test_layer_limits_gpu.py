@@ -44,3 +44,17 @@ def test_combine_gradients_of_the_longest_rows(dev):
     assert_same(dy[0], lambda s: torch.zeros_like(d[s]))
     assert float(dw) == 0
     assert bool((guard[:2048] == 9).all()) and bool((guard[2048 + N:] == 9).all())
+
+
+def test_dense_copies_the_longest_lines(dev):
+    """One line of 2^31 - 1 weights off a 16-byte boundary, which is copied to the
+    workspace; one token of one input, so that each output is one product."""
+    M = 2 ** 31 - 1
+    A = uniform(M + 1, dev, 3)[1:].view(1, M)
+    B = torch.full((1, 1), 0.75, dtype=torch.float16, device=dev)
+    guard = torch.full((M + 4097,), 9.0, dtype=torch.float16, device=dev)
+    C = guard[2048:2048 + M].view(1, M)
+    ops.dense(A, B, out=C)
+    ops.check_device()
+    assert_same(C[0], lambda s: (A[0, s].float() * 0.75).half())
+    assert bool((guard[:2048] == 9).all()) and bool((guard[2048 + M:] == 9).all())
