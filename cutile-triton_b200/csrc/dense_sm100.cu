@@ -653,8 +653,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     uint64_t* rbar = r_full + 2 * w;
     const uint32_t tmem_empty_leader = mapa_shared(smem_u32(&tmem_empty[0]), 0);
     const Epilogue& e = a.e;
-    const bool all_tma = a.d_tma && (!e.Z || a.z_tma);
     int sbuf = 0;
+    bool by_bulk = false;  // the last box was stored by TMA
     uint32_t r_issued = 0, r_used = 0;  // residual boxes asked for and read
     int it = 0;
 
@@ -670,12 +670,17 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     auto put = [&](const uint32_t (&v)[32], const CUtensorMap* map, void* base, int64_t ld,
                    bool tma, int r0, int c) {
       uint8_t* b = box + sbuf * PR_BOX;
-      // This box's previous store has read it: the last store but one where all
-      // go by TMA, else possibly the last.
+      // A TMA store ends a row at a 16-byte boundary (measured: columns of a row's
+      // last run that are past the matrix are written too), so the last chunk of
+      // rows that end elsewhere is stored by the warp.
+      tma = tma && (e.cols % 8 == 0 || e.cols - c >= 32);
+      // This box's previous store has read it: the last bulk store but one where
+      // the box between went by TMA, else possibly the last.
       if (lane == 0) {
-        if (all_tma) bulk_wait_read<1>();
+        if (by_bulk) bulk_wait_read<1>();
         else bulk_wait_read<0>();
       }
+      by_bulk = tma;
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
