@@ -672,7 +672,9 @@ static int gemm_f16_dispatch(const __half* A, const __half* B, __half* C, int M,
       return rc;
   }
   CUtensorMap tmC;
-  const bool c_tma = tma_ok(C, ldc, sC, batch);
+  // A TMA store rounds a column's end up to 16 bytes, so columns that end elsewhere
+  // (in padded storage) are written element by element.
+  const bool c_tma = M % 8 == 0 && tma_ok(C, ldc, sC, batch);
   if (c_tma) {
     const uint64_t dims[3] = {(uint64_t)M, (uint64_t)N, (uint64_t)batch};
     const uint64_t strides[2] = {(uint64_t)ldc * 2,
