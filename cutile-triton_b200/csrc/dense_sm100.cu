@@ -715,7 +715,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       const int r0 = tr * 256 + (int)rank * 128 + q * 32;
       const int c0 = tc * 256 + half * 128;
       // Chunks of this tile that hold any of D (a prefix of the four).
-      const int chunks = r0 < e.rows && c0 < e.cols ? min(4, (e.cols - c0 + 31) / 32) : 0;
+      const int chunks =
+          r0 < e.rows && c0 < e.cols ? (int)min(4u, ((uint32_t)(e.cols - c0) + 31) / 32) : 0;
       const bool by_tma = e.R && a.r_tma;
       if (by_tma)
         for (int i = 0; i < min(2, chunks); ++i) fetch_residual(r0, c0 + 32 * i);
