@@ -197,9 +197,10 @@ __device__ __forceinline__ void slope2(float& a, float& b) {
     const f2 z = mk2(a, b), zz = mul2(z, z);
     const f2 s = logistic_ex2(mul2(z, fma2(zz, all2(-kLog2e * kGeluScale * kGeluCube),
                                            all2(-kLog2e * kGeluScale))));
-    const f2 du = fma2(zz, all2(3.f * kGeluCube * kGeluScale), all2(kGeluScale));
     const f2 w = mul2(mul2(z, s), fma2(s, all2(-1.f), all2(1.f)));
-    un2(fma2(w, du, s), a, b);
+    float ua, ub;  // du/dz, kept finite where z^2 is not: w has long been 0 there
+    un2(fma2(zz, all2(3.f * kGeluCube * kGeluScale), all2(kGeluScale)), ua, ub);
+    un2(fma2(w, mk2(fminf(ua, 3e38f), fminf(ub, 3e38f)), s), a, b);
   } else {
     a = b = 1.f;
   }

@@ -13,7 +13,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.mark.parametrize("pair", ["1", "0"])
-@pytest.mark.parametrize("tests", ["test_dense_guards_gpu.py",
+@pytest.mark.parametrize("tests", ["test_dense_guards_gpu.py test_dense_values_gpu.py",
                                    "test_layer_limits_gpu.py -k longest_lines"])
 def test_forced_kernel(pair, tests):
     r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", *tests.split(),
