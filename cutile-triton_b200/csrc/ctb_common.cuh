@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/cutile_b200.h"
@@ -30,6 +31,30 @@ inline int launch_status(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, what);
   return CTB_OK;
+}
+
+// ---- operands that may not share memory ------------------------------------------
+// `rows` lines of `len` bytes, `pitch` bytes apart. Nothing where p is NULL.
+struct Lines {
+  const void* p;
+  int64_t rows, len, pitch;
+};
+// A matrix of elements of `size` bytes whose lines are `ld` elements apart.
+inline Lines lines_of(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t size) {
+  return {p, rows, cols * size, rows > 1 ? ld * size : cols * size};
+}
+inline Lines bytes_of(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+// Whether any byte belongs to both. Lines that lie between one another's (columns
+// of one wider buffer, every other row of it) do not overlap.
+bool overlap(const Lines& a, const Lines& b);
+inline bool apart(const Lines& a, std::initializer_list<Lines> others) {
+  for (const Lines& o : others)
+    if (overlap(a, o)) return false;
+  return true;
+}
+// The same lines at the same place: what an output that may be an input is held to.
+inline bool same_place(const Lines& a, const Lines& b) {
+  return a.p == b.p && a.rows == b.rows && a.len == b.len && a.pitch == b.pitch;
 }
 
 struct DeviceProps {

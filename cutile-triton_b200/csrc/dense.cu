@@ -373,9 +373,15 @@ extern "C" int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const 
     return set_error(CTB_ERR_LAYOUT, "dense: leading dimension smaller than the column length");
   if (M == 0 || N == 0) return CTB_OK;
   if (!C || (K > 0 && (!A || !B))) return set_error(CTB_ERR_ARG, "dense: NULL pointer");
-  if (C == A || C == B || (Z && (Z == C || Z == R || Z == A || Z == B)))
-    return set_error(CTB_ERR_ARG, "dense: C and Z must be matrices of their own (C may be R)");
   const int64_t need = ctb_dense_fwd_workspace_bytes(A, B, M, N, K, lda, ldb);
+  const Lines a = lines_of(A, K, M, lda, 2), b = lines_of(B, N, K, ldb, 2),
+              bi = bytes_of(bias, (bias_dtype == CTB_F32 ? 4ll : 2ll) * M),
+              r = lines_of(R, N, M, ldr, 2), z = lines_of(Z, N, M, ldz, 2),
+              c = lines_of(C, N, M, ldc, 2), w = bytes_of(workspace, need);
+  if (!apart(c, {a, b, bi, z, w}) || !(same_place(c, r) || apart(c, {r})) ||
+      !apart(z, {a, b, bi, r, w}) || !apart(w, {a, b, bi, r}))
+    return set_error(CTB_ERR_ARG, "dense: C, Z and the workspace must be memory of their own (C may "
+                                  "be R, with the same leading dimension)");
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return set_error(CTB_ERR_ARG, "dense: the workspace needs " + std::to_string(need) +
                                       " bytes, 16-byte aligned");
@@ -421,13 +427,18 @@ extern "C" int ctb_dense_bwd(int32_t dtype, const void* dC, const void* A, const
   const bool some = M > 0 && N > 0;
   if ((some && (!dC || (slope && !Z))) || (some && K > 0 && ((dB && !A) || (dA && !B))))
     return set_error(CTB_ERR_ARG, "dense_bwd: NULL pointer");
-  for (const void* out : {(const void*)dA, (const void*)dB, (const void*)dbias})
-    if (out && (out == dC || out == A || out == B || out == Z))
-      return set_error(CTB_ERR_ARG, "dense_bwd: gradients must be matrices of their own");
-  if (dA && dA == dB)
-    return set_error(CTB_ERR_ARG, "dense_bwd: gradients must be matrices of their own");
   const int64_t need = ctb_dense_bwd_workspace_bytes(dC, A, B, M, N, K, lddc, lda, ldb, act,
                                                      dbias != nullptr);
+  // Operands that are read: Z where there is an activation, A for dB, B for dA.
+  const Lines c = lines_of(dC, N, M, lddc, 2), z = lines_of(slope ? Z : nullptr, N, M, ldz, 2),
+              a = lines_of(dB ? A : nullptr, K, M, lda, 2),
+              b = lines_of(dA ? B : nullptr, N, K, ldb, 2), oa = lines_of(dA, K, M, ldda, 2),
+              ob = lines_of(dB, N, K, lddb, 2), obi = bytes_of(dbias, 4ll * M),
+              w = bytes_of(workspace, need);
+  if (!apart(oa, {c, z, a, b, ob, obi, w}) || !apart(ob, {c, z, a, b, obi, w}) ||
+      !apart(obi, {c, z, a, b, w}) || !apart(w, {c, z, a, b}))
+    return set_error(CTB_ERR_ARG,
+                     "dense_bwd: gradients and the workspace must be memory of their own");
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return set_error(CTB_ERR_ARG, "dense_bwd: the workspace needs " + std::to_string(need) +
                                       " bytes, 16-byte aligned");

@@ -293,8 +293,12 @@ extern "C" int ctb_moe_combine(int32_t dtype, const void* y, const float* weight
     return set_error(CTB_ERR_LAYOUT, "moe_combine: row stride smaller than the row");
   if (T == 0 || N == 0) return CTB_OK;
   if (!y || !out) return set_error(CTB_ERR_ARG, "moe_combine: NULL pointer");
-  if (out == y && topk > 1)
-    return set_error(CTB_ERR_ARG, "moe_combine: out over y needs one slot per token");
+  const Lines o = lines_of(out, T, N, ldo, 2), r = lines_of(residual, T, N, ldr, 2),
+              ys = lines_of(y, (int64_t)T * topk, N, ldy, 2);
+  if (!apart(o, {bytes_of(weights, 4ll * T * topk), bytes_of(ids, 4ll * T * topk)}) ||
+      !(same_place(o, r) || apart(o, {r})) || !((topk == 1 && same_place(o, ys)) || apart(o, {ys})))
+    return set_error(CTB_ERR_ARG, "moe_combine: out must be memory of its own (or the residual, or y "
+                                  "where topk is 1, with the same row stride)");
   DeviceProps pr;
   if (int rc = current_props(&pr)) return rc;
   auto st = static_cast<cudaStream_t>(stream);
@@ -327,8 +331,16 @@ extern "C" int ctb_moe_combine_bwd(int32_t dtype, const void* dout, const void* 
   if (T == 0) return CTB_OK;
   if ((N > 0 && (!dout || !dy)) || (weights && (!dweights || (N > 0 && !y))))
     return set_error(CTB_ERR_ARG, "moe_combine_bwd: NULL pointer");
-  if (dy == dout && N > 0 && topk > 1)
-    return set_error(CTB_ERR_ARG, "moe_combine_bwd: dy over dout needs one slot per token");
+  const int64_t slots = (int64_t)T * topk;
+  const Lines d = lines_of(dout, T, N, lddo, 2), ys = lines_of(weights ? y : nullptr, slots, N, ldy, 2),
+              dys = lines_of(dy, slots, N, lddy, 2), w = bytes_of(weights, 4 * slots),
+              i = bytes_of(ids, 4 * slots), dw = bytes_of(weights ? dweights : nullptr, 4 * slots);
+  if (!apart(dys, {w, i, dw}) || !(same_place(dys, ys) || apart(dys, {ys})) ||
+      !((topk == 1 && same_place(dys, d)) || apart(dys, {d})) || !apart(dw, {d, ys, i}) ||
+      !(same_place(dw, w) || apart(dw, {w})))
+    return set_error(CTB_ERR_ARG, "moe_combine_bwd: dy and dweights must be memory of their own (dy "
+                                  "may be y, or dout where topk is 1, with the same row stride; "
+                                  "dweights may be the weights)");
   DeviceProps pr;
   if (int rc = current_props(&pr)) return rc;
   auto st = static_cast<cudaStream_t>(stream);

@@ -862,6 +862,11 @@ extern "C" int ctb_moe_route(int32_t dtype, const void* logits, const float* bia
     return set_error(CTB_ERR_SHAPE, "moe_route: topk exceeds the experts of topk_groups groups");
   if (T == 0) return CTB_OK;
   if (!logits || !weights || !ids) return set_error(CTB_ERR_ARG, "moe_route: NULL pointer");
+  const int size = dtype == CTB_F32 ? 4 : 2;
+  const Lines x = lines_of(logits, T, E, ldx, size), b = bytes_of(bias, 4ll * E),
+              w = bytes_of(weights, 4ll * T * topk), i = bytes_of(ids, 4ll * T * topk);
+  if (!apart(w, {x, b, i}) || !apart(i, {x, b}))
+    return set_error(CTB_ERR_ARG, "moe_route: weights and ids must be memory of their own");
   DeviceProps pr;
   if (int rc = current_props(&pr)) return rc;
   RouteArgs a = {};
@@ -897,6 +902,12 @@ extern "C" int ctb_moe_route_bwd(int32_t dtype, const float* dweights, const voi
   if (T == 0) return CTB_OK;
   if (!dweights || !logits || !ids || !dlogits)
     return set_error(CTB_ERR_ARG, "moe_route_bwd: NULL pointer");
+  const int size = dtype == CTB_F32 ? 4 : 2;
+  const Lines x = lines_of(logits, T, E, ldx, size), dx = lines_of(dlogits, T, E, lddx, size);
+  if (!apart(dx, {bytes_of(dweights, 4ll * T * topk), bytes_of(ids, 4ll * T * topk)}) ||
+      !(same_place(dx, x) || apart(dx, {x})))
+    return set_error(CTB_ERR_ARG, "moe_route_bwd: dlogits must be memory of its own (or the logits, "
+                                  "with the same row stride)");
   DeviceProps pr;
   if (int rc = current_props(&pr)) return rc;
   RouteBwdArgs a;

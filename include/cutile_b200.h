@@ -312,9 +312,10 @@ typedef enum {
  * column-major: A is M x K (the weight), B is K x N (a column per token), C,
  * R and Z are M x N; lda, ldb, ldr, ldz, ldc are column strides. bias: M
  * elements of dtype bias_dtype (the matrices' or F32), or NULL; R (residual)
- * may be NULL, and may be C itself; Z receives the value before the
- * activation (what ctb_dense_bwd needs), or is NULL. Nothing else may overlap
- * what is written. Sums, bias, activation and residual are Float32, rounded
+ * may be NULL, and may be C itself (with ldr = ldc); Z receives the value
+ * before the activation (what ctb_dense_bwd needs), or is NULL. Nothing else
+ * may share a byte with what is written, the workspace included (refused;
+ * columns of one wider buffer do not). Sums, bias, activation and residual are Float32, rounded
  * once to C (and once to Z); no atomics, so a call's result is always the
  * same. `workspace` (16-byte aligned) of at least
  * ctb_dense_fwd_workspace_bytes() bytes, which is 0 when A and B start on
@@ -331,7 +332,8 @@ int ctb_dense_fwd(int32_t dtype, const void* A, const void* B, const void* bias,
  * Any of dA, dB, dbias may be NULL (not wanted). Z is the forward call's (not
  * read where act is CTB_ACT_NONE). The gradient of the residual is dC. dZ is
  * rounded to the matrices' type as an operand of the products; dbias is summed
- * in Float32 from the unrounded values, in a fixed order. */
+ * in Float32 from the unrounded values, in a fixed order. What is written
+ * shares no byte with anything else (refused). */
 int64_t ctb_dense_bwd_workspace_bytes(const void* dC, const void* A, const void* B, int32_t M,
                                       int32_t N, int32_t K, int64_t lddc, int64_t lda,
                                       int64_t ldb, int32_t act, int32_t need_dbias);
@@ -371,7 +373,8 @@ int ctb_moe_route(int32_t dtype, const void* logits, const float* bias, float* w
 /* Gradient of ctb_moe_route's weights with respect to the logits: dlogits
  * (T x E, row stride lddx, dtype of the logits) from dweights (T x topk) and
  * the ids that the forward call gave; `score`, `renorm` and `scale` as there.
- * Places with an id outside [0, E) or a logit of -inf or NaN give nothing. */
+ * Places with an id outside [0, E) or a logit of -inf or NaN give nothing.
+ * dlogits may be the logits themselves (with lddx = ldx). */
 int ctb_moe_route_bwd(int32_t dtype, const float* dweights, const void* logits,
                       const int32_t* ids, void* dlogits, int32_t T, int32_t E, int32_t topk,
                       int64_t ldx, int64_t lddx, int32_t score, int32_t renorm, float scale,
@@ -383,7 +386,8 @@ int ctb_moe_route_bwd(int32_t dtype, const float* dweights, const void* logits,
  * contiguous elements, dtype F16 or BF16, row stride ldy; weights: T x topk
  * floats or NULL (all 1: ctb_moe_gemm_f16 may have applied them); residual:
  * row stride ldr, or NULL; out: row stride ldo, may be the residual itself
- * (and y itself where topk is 1).
+ * (and y itself where topk is 1), with the same row stride; any other overlap
+ * is refused.
  * ids: T x topk or NULL; a slot whose id is outside [0, E) was given to no
  * expert: its row of y is not read and its weight not used. */
 int ctb_moe_combine(int32_t dtype, const void* y, const float* weights, const int32_t* ids,
@@ -394,7 +398,9 @@ int ctb_moe_combine(int32_t dtype, const void* y, const float* weights, const in
  * dweights[t, j] = sum_n dout[t, n] * y[t * topk + j, n] (Float32). Slots with
  * an id outside [0, E) get zeros in both, their rows of y are not read. With
  * weights NULL, y and dweights are not used and may be NULL. The gradient of
- * the residual is dout itself. */
+ * the residual is dout itself. dy may be y itself (and dout where topk is 1),
+ * with the same row stride, dweights may be weights; any other overlap is
+ * refused. */
 int ctb_moe_combine_bwd(int32_t dtype, const void* dout, const void* y, const float* weights,
                         const int32_t* ids, void* dy, float* dweights, int32_t T, int32_t topk,
                         int32_t N, int32_t E, int64_t lddo, int64_t ldy, int64_t lddy,
