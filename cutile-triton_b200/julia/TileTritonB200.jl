@@ -332,14 +332,17 @@ function moe_align(topk_ids::CuMatrix{Int32}, num_experts::Integer; block::Integ
 end
 
 # ---------------------------------------------------------------------------- layer calls
-const F16s = Union{Float16,Core.BFloat16}
 const ACTS = Dict(:none => 0, :relu => 1, :gelu => 2, :gelu_tanh => 3, :silu => 4)
 const SCORES = Dict(:softmax => 0, :sigmoid => 1)
 ldim(x) = stride(x, 2)
 orC(x) = x === nothing ? CU_NULL : pointer(x)
-codeof(::Type{Float16}) = Int32(1)
-codeof(::Type{Core.BFloat16}) = Int32(2)
-codeof(::Type{Float32}) = Int32(3)
+# The 16-bit types of the layer calls. BFloat16 is known by its name: it is Core's
+# from Julia 1.11 on and a package's before.
+function layer_code(what::String, T::Type)
+    c = dtype_code(T)
+    c == 1 || c == 2 || error("b200: $what: matrices must be Float16 or BFloat16, got $T")
+    return c
+end
 
 """
     dense!(C, A, B; bias=nothing, act=:none, R=nothing, Z=nothing)
@@ -350,7 +353,7 @@ weight, B (K, N) a column per token; `act` one of :none, :relu, :gelu,
 before the activation (`ctb_dense_fwd`).
 """
 function dense!(C::StridedCuMatrix{T}, A::StridedCuMatrix{T}, B::StridedCuMatrix{T}; bias=nothing,
-                act::Symbol=:none, R=nothing, Z=nothing) where {T<:F16s}
+                act::Symbol=:none, R=nothing, Z=nothing) where {T}
     M, K = size(A)
     N = size(B, 2)
     size(B, 1) == K && size(C) == (M, N) || error("b200: dense!: sizes disagree")
@@ -361,7 +364,7 @@ function dense!(C::StridedCuMatrix{T}, A::StridedCuMatrix{T}, B::StridedCuMatrix
                 (Int32, CuPtr{T}, CuPtr{T}, CuPtr{Cvoid}, Int32, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{T},
                  Int32, Int32, Int32, Int64, Int64, Int64, Int64, Int64, Int32, CuPtr{UInt8}, Int64,
                  Ptr{Cvoid}),
-                codeof(T), A, B, orC(bias), bias === nothing ? 0 : codeof(eltype(bias)), orC(R), orC(Z),
+                layer_code("dense!", T), A, B, orC(bias), bias === nothing ? 0 : dtype_code(eltype(bias)), orC(R), orC(Z),
                 C, M, N, K, ldim(A), ldim(B), R === nothing ? 0 : ldim(R), Z === nothing ? 0 : ldim(Z),
                 ldim(C), ACTS[act], ws, nws, CUDA.stream().handle))
     return C
@@ -374,7 +377,7 @@ Gradients of `dense!` from dC (M, N); any of dA (M, K), dB (K, N), dbias (M,
 Float32) may be `nothing`. Z is the forward call's (`ctb_dense_bwd`).
 """
 function dense_bwd!(dA, dB, dbias, dC::StridedCuMatrix{T}, A::StridedCuMatrix{T}, B::StridedCuMatrix{T};
-                    act::Symbol=:none, Z=nothing) where {T<:F16s}
+                    act::Symbol=:none, Z=nothing) where {T}
     M, K = size(A)
     N = size(B, 2)
     size(B, 1) == K && size(dC) == (M, N) || error("b200: dense_bwd!: sizes disagree")
@@ -386,7 +389,7 @@ function dense_bwd!(dA, dB, dbias, dC::StridedCuMatrix{T}, A::StridedCuMatrix{T}
                 (Int32, CuPtr{T}, CuPtr{T}, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid},
                  CuPtr{Cvoid}, Int32, Int32, Int32, Int64, Int64, Int64, Int64, Int64, Int64, Int32,
                  CuPtr{UInt8}, Int64, Ptr{Cvoid}),
-                codeof(T), dC, A, B, orC(Z), orC(dA), orC(dB), orC(dbias), M, N, K, ldim(dC), ldim(A),
+                layer_code("dense_bwd!", T), dC, A, B, orC(Z), orC(dA), orC(dB), orC(dbias), M, N, K, ldim(dC), ldim(A),
                 ldim(B), Z === nothing ? 0 : ldim(Z), dA === nothing ? 0 : ldim(dA),
                 dB === nothing ? 0 : ldim(dB), ACTS[act], ws, nws, CUDA.stream().handle))
     return dA, dB, dbias
@@ -402,27 +405,27 @@ weights Float32 and 0-based ids Int32, both (topk, T), for `moe_align` and the
 """
 function moe_route(logits::StridedCuMatrix{T}, topk::Integer; score::Symbol=:softmax, bias=nothing,
                    groups::Integer=1, topk_groups::Integer=groups, group_top::Integer=2,
-                   renorm::Bool=true, scale::Real=1) where {T<:Union{F16s,Float32}}
+                   renorm::Bool=true, scale::Real=1) where {T}
     E, n = size(logits)
     weights, ids = CuArray{Float32}(undef, topk, n), CuArray{Int32}(undef, topk, n)
     GC.@preserve bias check(ccall(sym(:ctb_moe_route), Cint,
                 (Int32, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Float32}, CuPtr{Int32}, Int32, Int32, Int32, Int64,
                  Int32, Int32, Int32, Int32, Int32, Float32, Ptr{Cvoid}),
-                codeof(T), logits, orC(bias), weights, ids, n, E, topk, ldim(logits), SCORES[score],
+                dtype_code(T), logits, orC(bias), weights, ids, n, E, topk, ldim(logits), SCORES[score],
                 groups, topk_groups, group_top, renorm, scale, CUDA.stream().handle))
     return weights, ids
 end
 
 "Gradient of `moe_route`'s weights with respect to the logits, for the ids it gave (`ctb_moe_route_bwd`)."
 function moe_route_bwd(dweights::CuMatrix{Float32}, logits::StridedCuMatrix{T}, ids::CuMatrix{Int32};
-                       score::Symbol=:softmax, renorm::Bool=true, scale::Real=1) where {T<:Union{F16s,Float32}}
+                       score::Symbol=:softmax, renorm::Bool=true, scale::Real=1) where {T}
     E, n = size(logits)
     size(ids, 2) == n && size(dweights) == size(ids) || error("b200: moe_route_bwd: sizes disagree")
     dlogits = CuArray{T}(undef, E, n)
     check(ccall(sym(:ctb_moe_route_bwd), Cint,
                 (Int32, CuPtr{Float32}, CuPtr{T}, CuPtr{Int32}, CuPtr{T}, Int32, Int32, Int32, Int64, Int64,
                  Int32, Int32, Float32, Ptr{Cvoid}),
-                codeof(T), dweights, logits, ids, dlogits, n, E, size(ids, 1), ldim(logits), E,
+                dtype_code(T), dweights, logits, ids, dlogits, n, E, size(ids, 1), ldim(logits), E,
                 SCORES[score], renorm, scale, CUDA.stream().handle))
     return dlogits
 end
@@ -434,27 +437,27 @@ out[:, t] = R[:, t] + sum over j of weights[j, t] * y[:, (t - 1) topk + j], slot
 with an id outside 0:num_experts-1 left out (`ctb_moe_combine`).
 """
 function moe_combine!(out::StridedCuMatrix{T}, y::StridedCuMatrix{T}, topk::Integer; weights=nothing,
-                      ids=nothing, num_experts::Integer=0, R=nothing) where {T<:F16s}
+                      ids=nothing, num_experts::Integer=0, R=nothing) where {T}
     N, n = size(out)
     size(y) == (N, n * topk) || error("b200: moe_combine!: sizes disagree")
     GC.@preserve weights ids R check(ccall(sym(:ctb_moe_combine), Cint,
                 (Int32, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{T}, Int32, Int32, Int32,
                  Int32, Int64, Int64, Int64, Ptr{Cvoid}),
-                codeof(T), y, orC(weights), orC(ids), orC(R), out, n, topk, N, num_experts, ldim(y),
+                layer_code("moe_combine!", T), y, orC(weights), orC(ids), orC(R), out, n, topk, N, num_experts, ldim(y),
                 R === nothing ? 0 : ldim(R), ldim(out), CUDA.stream().handle))
     return out
 end
 
 "Gradients (dy, dweights) of `moe_combine!` from dout (N, T) (`ctb_moe_combine_bwd`)."
 function moe_combine_bwd(dout::StridedCuMatrix{T}, y, topk::Integer; weights=nothing, ids=nothing,
-                         num_experts::Integer=0) where {T<:F16s}
+                         num_experts::Integer=0) where {T}
     N, n = size(dout)
     dy = CuArray{T}(undef, N, n * topk)
     dweights = weights === nothing ? nothing : CuArray{Float32}(undef, topk, n)
     GC.@preserve y weights ids dweights check(ccall(sym(:ctb_moe_combine_bwd), Cint,
                 (Int32, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{T}, CuPtr{Cvoid}, Int32,
                  Int32, Int32, Int32, Int64, Int64, Int64, Ptr{Cvoid}),
-                codeof(T), dout, weights === nothing ? CU_NULL : pointer(y), orC(weights), orC(ids), dy,
+                layer_code("moe_combine_bwd", T), dout, weights === nothing ? CU_NULL : pointer(y), orC(weights), orC(ids), dy,
                 orC(dweights), n, topk, N, num_experts, ldim(dout), weights === nothing ? 0 : ldim(y), N,
                 CUDA.stream().handle))
     return dy, dweights
