@@ -334,8 +334,28 @@ end
 # ---------------------------------------------------------------------------- layer calls
 const ACTS = Dict(:none => 0, :relu => 1, :gelu => 2, :gelu_tanh => 3, :silu => 4)
 const SCORES = Dict(:softmax => 0, :sigmoid => 1)
-ldim(x) = stride(x, 2)
+# The column stride that the C ABI is given; one column has none that matters.
+ldim(x) = size(x, 2) > 1 ? stride(x, 2) : max(size(x, 1), 1)
+ldor0(x) = x === nothing ? 0 : ldim(x)
 orC(x) = x === nothing ? CU_NULL : pointer(x)
+
+"""
+    operand(x, what, T, dims; packed=false)
+
+What the library cannot see in a pointer: that `x` (or `nothing`) is a device
+array of element type `T` and size `dims` whose columns are contiguous, and with
+`packed` follow one another.
+"""
+function operand(x, what::String, T::Type, dims::Dims; packed::Bool=false)
+    x === nothing && return nothing
+    x isa StridedCuArray || error("b200: $what: expected a device array, got $(typeof(x))")
+    eltype(x) === T || error("b200: $what: expected elements of type $T, got $(eltype(x))")
+    size(x) == dims || error("b200: $what: expected size $dims, got $(size(x))")
+    size(x, 1) <= 1 || stride(x, 1) == 1 || error("b200: $what: columns must be contiguous")
+    packed && length(dims) == 2 && ldim(x) != max(dims[1], 1) && error("b200: $what: must be contiguous")
+    return nothing
+end
+
 # The 16-bit types of the layer calls. BFloat16 is known by its name: it is Core's
 # from Julia 1.11 on and a package's before.
 function layer_code(what::String, T::Type)
@@ -343,6 +363,8 @@ function layer_code(what::String, T::Type)
     c == 1 || c == 2 || error("b200: $what: matrices must be Float16 or BFloat16, got $T")
     return c
 end
+choice(table, key::Symbol, what::String) =
+    get(() -> error("b200: $what: none of $(join(keys(table), ", "))"), table, key)
 
 """
     dense!(C, A, B; bias=nothing, act=:none, R=nothing, Z=nothing)
@@ -354,9 +376,16 @@ before the activation (`ctb_dense_fwd`).
 """
 function dense!(C::StridedCuMatrix{T}, A::StridedCuMatrix{T}, B::StridedCuMatrix{T}; bias=nothing,
                 act::Symbol=:none, R=nothing, Z=nothing) where {T}
+    code = layer_code("dense!", T)
     M, K = size(A)
     N = size(B, 2)
-    size(B, 1) == K && size(C) == (M, N) || error("b200: dense!: sizes disagree")
+    operand(A, "dense!: A", T, (M, K))
+    operand(B, "dense!: B", T, (K, N))
+    operand(C, "dense!: C", T, (M, N))
+    operand(bias, "dense!: bias", bias isa AbstractArray{Float32} ? Float32 : T, (M,))
+    operand(R, "dense!: R", T, (M, N))
+    operand(Z, "dense!: Z", T, (M, N))
+    a = choice(ACTS, act, "dense!: act")
     nws = ccall(sym(:ctb_dense_fwd_workspace_bytes), Int64,
                 (CuPtr{T}, CuPtr{T}, Int32, Int32, Int32, Int64, Int64), A, B, M, N, K, ldim(A), ldim(B))
     ws = CuArray{UInt8}(undef, max(nws, 1))
@@ -364,9 +393,9 @@ function dense!(C::StridedCuMatrix{T}, A::StridedCuMatrix{T}, B::StridedCuMatrix
                 (Int32, CuPtr{T}, CuPtr{T}, CuPtr{Cvoid}, Int32, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{T},
                  Int32, Int32, Int32, Int64, Int64, Int64, Int64, Int64, Int32, CuPtr{UInt8}, Int64,
                  Ptr{Cvoid}),
-                layer_code("dense!", T), A, B, orC(bias), bias === nothing ? 0 : dtype_code(eltype(bias)), orC(R), orC(Z),
-                C, M, N, K, ldim(A), ldim(B), R === nothing ? 0 : ldim(R), Z === nothing ? 0 : ldim(Z),
-                ldim(C), ACTS[act], ws, nws, CUDA.stream().handle))
+                code, A, B, orC(bias), bias === nothing ? 0 : dtype_code(eltype(bias)), orC(R), orC(Z),
+                C, M, N, K, ldim(A), ldim(B), ldor0(R), ldor0(Z), ldim(C), a, ws, nws,
+                CUDA.stream().handle))
     return C
 end
 
@@ -378,20 +407,27 @@ Float32) may be `nothing`. Z is the forward call's (`ctb_dense_bwd`).
 """
 function dense_bwd!(dA, dB, dbias, dC::StridedCuMatrix{T}, A::StridedCuMatrix{T}, B::StridedCuMatrix{T};
                     act::Symbol=:none, Z=nothing) where {T}
+    code = layer_code("dense_bwd!", T)
     M, K = size(A)
     N = size(B, 2)
-    size(B, 1) == K && size(dC) == (M, N) || error("b200: dense_bwd!: sizes disagree")
+    operand(dC, "dense_bwd!: dC", T, (M, N))
+    operand(A, "dense_bwd!: A", T, (M, K))
+    operand(B, "dense_bwd!: B", T, (K, N))
+    operand(Z, "dense_bwd!: Z", T, (M, N))
+    operand(dA, "dense_bwd!: dA", T, (M, K))
+    operand(dB, "dense_bwd!: dB", T, (K, N))
+    operand(dbias, "dense_bwd!: dbias", Float32, (M,))
+    a = choice(ACTS, act, "dense_bwd!: act")
     nws = ccall(sym(:ctb_dense_bwd_workspace_bytes), Int64,
                 (CuPtr{T}, CuPtr{T}, CuPtr{T}, Int32, Int32, Int32, Int64, Int64, Int64, Int32, Int32),
-                dC, A, B, M, N, K, ldim(dC), ldim(A), ldim(B), ACTS[act], dbias === nothing ? 0 : 1)
+                dC, A, B, M, N, K, ldim(dC), ldim(A), ldim(B), a, dbias === nothing ? 0 : 1)
     ws = CuArray{UInt8}(undef, max(nws, 1))
     GC.@preserve dA dB dbias dC A B Z ws check(ccall(sym(:ctb_dense_bwd), Cint,
                 (Int32, CuPtr{T}, CuPtr{T}, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid},
                  CuPtr{Cvoid}, Int32, Int32, Int32, Int64, Int64, Int64, Int64, Int64, Int64, Int32,
                  CuPtr{UInt8}, Int64, Ptr{Cvoid}),
-                layer_code("dense_bwd!", T), dC, A, B, orC(Z), orC(dA), orC(dB), orC(dbias), M, N, K, ldim(dC), ldim(A),
-                ldim(B), Z === nothing ? 0 : ldim(Z), dA === nothing ? 0 : ldim(dA),
-                dB === nothing ? 0 : ldim(dB), ACTS[act], ws, nws, CUDA.stream().handle))
+                code, dC, A, B, orC(Z), orC(dA), orC(dB), orC(dbias), M, N, K, ldim(dC), ldim(A),
+                ldim(B), ldor0(Z), ldor0(dA), ldor0(dB), a, ws, nws, CUDA.stream().handle))
     return dA, dB, dbias
 end
 
@@ -407,12 +443,16 @@ function moe_route(logits::StridedCuMatrix{T}, topk::Integer; score::Symbol=:sof
                    groups::Integer=1, topk_groups::Integer=groups, group_top::Integer=2,
                    renorm::Bool=true, scale::Real=1) where {T}
     E, n = size(logits)
+    topk >= 1 || error("b200: moe_route: topk must be positive")
+    operand(logits, "moe_route: logits", T, (E, n))
+    operand(bias, "moe_route: bias", Float32, (E,))
     weights, ids = CuArray{Float32}(undef, topk, n), CuArray{Int32}(undef, topk, n)
     GC.@preserve bias check(ccall(sym(:ctb_moe_route), Cint,
                 (Int32, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Float32}, CuPtr{Int32}, Int32, Int32, Int32, Int64,
                  Int32, Int32, Int32, Int32, Int32, Float32, Ptr{Cvoid}),
-                dtype_code(T), logits, orC(bias), weights, ids, n, E, topk, ldim(logits), SCORES[score],
-                groups, topk_groups, group_top, renorm, scale, CUDA.stream().handle))
+                dtype_code(T), logits, orC(bias), weights, ids, n, E, topk, ldim(logits),
+                choice(SCORES, score, "moe_route: score"), groups, topk_groups, group_top, renorm, scale,
+                CUDA.stream().handle))
     return weights, ids
 end
 
@@ -420,13 +460,16 @@ end
 function moe_route_bwd(dweights::CuMatrix{Float32}, logits::StridedCuMatrix{T}, ids::CuMatrix{Int32};
                        score::Symbol=:softmax, renorm::Bool=true, scale::Real=1) where {T}
     E, n = size(logits)
-    size(ids, 2) == n && size(dweights) == size(ids) || error("b200: moe_route_bwd: sizes disagree")
+    topk = size(ids, 1)
+    operand(logits, "moe_route_bwd: logits", T, (E, n))
+    operand(ids, "moe_route_bwd: ids", Int32, (topk, n); packed=true)
+    operand(dweights, "moe_route_bwd: dweights", Float32, (topk, n); packed=true)
     dlogits = CuArray{T}(undef, E, n)
     check(ccall(sym(:ctb_moe_route_bwd), Cint,
                 (Int32, CuPtr{Float32}, CuPtr{T}, CuPtr{Int32}, CuPtr{T}, Int32, Int32, Int32, Int64, Int64,
                  Int32, Int32, Float32, Ptr{Cvoid}),
-                dtype_code(T), dweights, logits, ids, dlogits, n, E, size(ids, 1), ldim(logits), E,
-                SCORES[score], renorm, scale, CUDA.stream().handle))
+                dtype_code(T), dweights, logits, ids, dlogits, n, E, topk, ldim(logits), E,
+                choice(SCORES, score, "moe_route_bwd: score"), renorm, scale, CUDA.stream().handle))
     return dlogits
 end
 
@@ -438,28 +481,41 @@ with an id outside 0:num_experts-1 left out (`ctb_moe_combine`).
 """
 function moe_combine!(out::StridedCuMatrix{T}, y::StridedCuMatrix{T}, topk::Integer; weights=nothing,
                       ids=nothing, num_experts::Integer=0, R=nothing) where {T}
+    code = layer_code("moe_combine!", T)
     N, n = size(out)
-    size(y) == (N, n * topk) || error("b200: moe_combine!: sizes disagree")
+    topk >= 1 || error("b200: moe_combine!: topk must be positive")
+    operand(out, "moe_combine!: out", T, (N, n))
+    operand(y, "moe_combine!: y", T, (N, Int(n * topk)))
+    operand(weights, "moe_combine!: weights", Float32, (Int(topk), n); packed=true)
+    operand(ids, "moe_combine!: ids", Int32, (Int(topk), n); packed=true)
+    operand(R, "moe_combine!: R", T, (N, n))
     GC.@preserve weights ids R check(ccall(sym(:ctb_moe_combine), Cint,
                 (Int32, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{T}, Int32, Int32, Int32,
                  Int32, Int64, Int64, Int64, Ptr{Cvoid}),
-                layer_code("moe_combine!", T), y, orC(weights), orC(ids), orC(R), out, n, topk, N, num_experts, ldim(y),
-                R === nothing ? 0 : ldim(R), ldim(out), CUDA.stream().handle))
+                code, y, orC(weights), orC(ids), orC(R), out, n, topk, N, num_experts, ldim(y), ldor0(R),
+                ldim(out), CUDA.stream().handle))
     return out
 end
 
 "Gradients (dy, dweights) of `moe_combine!` from dout (N, T) (`ctb_moe_combine_bwd`)."
 function moe_combine_bwd(dout::StridedCuMatrix{T}, y, topk::Integer; weights=nothing, ids=nothing,
                          num_experts::Integer=0) where {T}
+    code = layer_code("moe_combine_bwd", T)
     N, n = size(dout)
+    topk >= 1 || error("b200: moe_combine_bwd: topk must be positive")
+    weights === nothing || y !== nothing || error("b200: moe_combine_bwd: weights need y")
+    ys = weights === nothing ? nothing : y  # not used without weights
+    operand(dout, "moe_combine_bwd: dout", T, (N, n))
+    operand(ys, "moe_combine_bwd: y", T, (N, Int(n * topk)))
+    operand(weights, "moe_combine_bwd: weights", Float32, (Int(topk), n); packed=true)
+    operand(ids, "moe_combine_bwd: ids", Int32, (Int(topk), n); packed=true)
     dy = CuArray{T}(undef, N, n * topk)
     dweights = weights === nothing ? nothing : CuArray{Float32}(undef, topk, n)
-    GC.@preserve y weights ids dweights check(ccall(sym(:ctb_moe_combine_bwd), Cint,
+    GC.@preserve ys weights ids dweights check(ccall(sym(:ctb_moe_combine_bwd), Cint,
                 (Int32, CuPtr{T}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{T}, CuPtr{Cvoid}, Int32,
                  Int32, Int32, Int32, Int64, Int64, Int64, Ptr{Cvoid}),
-                layer_code("moe_combine_bwd", T), dout, weights === nothing ? CU_NULL : pointer(y), orC(weights), orC(ids), dy,
-                orC(dweights), n, topk, N, num_experts, ldim(dout), weights === nothing ? 0 : ldim(y), N,
-                CUDA.stream().handle))
+                code, dout, orC(ys), orC(weights), orC(ids), dy, orC(dweights), n, topk, N, num_experts,
+                ldim(dout), ldor0(ys), max(N, 1), CUDA.stream().handle))
     return dy, dweights
 end
 

@@ -110,4 +110,36 @@ let n = 1000, m = 2048
     check("vadd_host! (bit-exact)", c == a .+ b)
 end
 
+let M = 40, N = 6, K = 24
+    A = CUDA.rand(Float16, M, K); B = CUDA.rand(Float16, K, N); bias = CUDA.rand(Float32, M)
+    R = CUDA.rand(Float16, M, N); C = CUDA.zeros(Float16, M, N); Z = CUDA.zeros(Float16, M, N)
+    TR.dense!(C, A, B; bias, act=:relu, R, Z)
+    z = Float64.(Array(A)) * Float64.(Array(B)) .+ Array(bias)
+    # K Float32 additions and the rounding of Z and C
+    check("dense! $M x $N x $K", maximum(abs.(Array(C) .- (max.(z, 0) .+ Array(R)))) <= 0.02)
+    weights, ids = TR.moe_route(CUDA.rand(Float32, 8, N), 2)
+    y = CUDA.rand(Float16, M, 2N); out = CUDA.zeros(Float16, M, N)
+    TR.moe_combine!(out, y, 2; weights, ids, num_experts=8)
+    refused(f) = try f(); false catch e; e isa ErrorException end
+    bad = CUDA.rand(Float16, M, 3)
+    check("layer calls refuse what the pointers would hide", all(refused, [
+        () -> TR.dense!(C, A, B; bias=CUDA.rand(Float32, M - 1)),
+        () -> TR.dense!(C, A, B; bias=CUDA.rand(Float64, M)),
+        () -> TR.dense!(C, A, B; R=bad), () -> TR.dense!(C, A, B; R=CUDA.rand(Float32, M, N)),
+        () -> TR.dense!(C, A, B; Z=bad), () -> TR.dense!(C, view(CUDA.rand(Float16, 2M, K), 1:2:2M, :), B),
+        () -> TR.dense!(C, A, B; act=:tanh),
+        () -> TR.dense_bwd!(bad, nothing, nothing, C, A, B), () -> TR.dense_bwd!(nothing, bad, nothing, C, A, B),
+        () -> TR.dense_bwd!(nothing, nothing, CUDA.zeros(Float32, M - 1), C, A, B),
+        () -> TR.dense_bwd!(nothing, nothing, CUDA.zeros(Float16, M), C, A, B),
+        () -> TR.dense_bwd!(similar(A), nothing, nothing, C, A, B; act=:relu, Z=bad),
+        () -> TR.moe_route(CUDA.rand(Float32, 8, N), 2; bias=CUDA.rand(Float32, 7)),
+        () -> TR.moe_route(CUDA.rand(Float32, 8, N), 2; bias=CUDA.rand(Float16, 8)),
+        () -> TR.moe_combine!(out, y, 2; weights=CUDA.rand(Float16, 2, N)),
+        () -> TR.moe_combine!(out, y, 2; weights, ids=CUDA.zeros(Int32, 2, N - 1), num_experts=8),
+        () -> TR.moe_combine!(out, y, 2; weights, R=bad),
+        () -> TR.moe_combine_bwd(out, bad, 2; weights), () -> TR.moe_combine_bwd(out, nothing, 2; weights),
+        () -> TR.moe_combine_bwd(out, y, 2; weights=CUDA.rand(Float32, 3, N)),
+    ]))
+end
+
 println("ALL $npass TESTS PASSED")
