@@ -163,41 +163,6 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
   return r;
 }
 
-__device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Writes 4 bytes to another CTA's shared memory, counted on a barrier of that CTA
-// (both by their shared::cluster addresses).
-__device__ __forceinline__ void st_async_cluster(uint32_t addr, uint32_t v, uint32_t bar) {
-  asm volatile(
-      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr),
-      "r"(v), "r"(bar)
-      : "memory");
-}
-// Waits (12 s at most, above the 4 s after which a sender gives its own pipeline
-// up) for what the cluster's CTAs send.
-__device__ __forceinline__ void wait_received(uint64_t* bar, volatile int* abort_flag) {
-  const uint64_t t0 = sm100::global_ns();
-  uint32_t ok = 0;
-  while (!ok) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(sm100::smem_u32(bar)), "r"(0u), "r"(20000u)
-        : "memory");
-    if (!ok && sm100::global_ns() - t0 > 12000000000ull) {
-      *abort_flag = 1;
-      flag_device_error(ERR_BIT);
-      return;
-    }
-  }
-}
-
 __device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&v)[32]) {
   sm100::tmem_ld_32x32b_x32(addr, v);
 }
@@ -384,9 +349,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2)
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
-  // Every CTA sends, also one whose pipeline gave up after its 4 s, so what this
-  // one waits for arrives before it may leave.
-  if (send && owned > 0) wait_received(received, abort_flag);
+  // Every CTA sends, also one whose pipeline gave up (after 4 s without progress).
+  if (send && owned > 0) wait_received(received, abort_flag, ERR_BIT, 12000000000ull);
 
   const uint32_t mine = smem_u32(partial);
   const int first_row = send ? (int)rank * each : 0, end_row = send ? first_row + owned : live_rows;

@@ -249,6 +249,60 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Writes 4 bytes to another CTA's shared memory, counted on a barrier of that CTA
+// (both by their shared::cluster addresses).
+__device__ __forceinline__ void st_async_cluster(uint32_t addr, uint32_t v, uint32_t bar) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr),
+      "r"(v), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ bool received_try_wait(uint64_t* bar) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(0u), "r"(20000u)
+      : "memory");
+  return ok;
+}
+// What a warp does whose wait for the other CTAs' sends gave up: the host is told,
+// and the warp stays until every other thread of the cluster has left (each has
+// sent its share by then; the barrier waits for threads that have not exited only)
+// and what is still in flight has landed, so that nothing is written to shared
+// memory that this CTA no longer holds. A sender has no limit for all of its work
+// that a receiver could go by: its waits are limited one by one.
+[[maybe_unused]] static __device__ __noinline__ void late_received(uint64_t* bar,
+                                                                   volatile int* abort_flag,
+                                                                   unsigned err_bit) {
+  *abort_flag = 1;
+  if (threadIdx.x % 32 == 0) flag_device_error(err_bit);
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  const uint64_t t0 = global_ns();
+  while (!received_try_wait(bar) && global_ns() - t0 < 1000000000ull) {
+  }
+}
+// Waits for what the cluster's CTAs send (first phase of `bar`), `limit_ns` at most.
+// Called by whole warps that have sent their own share, last but for work in
+// their own CTA's memory: no barrier of the cluster comes after it.
+__device__ __forceinline__ void wait_received(uint64_t* bar, volatile int* abort_flag,
+                                              unsigned err_bit, uint64_t limit_ns) {
+  const uint64_t t0 = global_ns();
+  bool ok = false;
+  while (!(ok = received_try_wait(bar)) && global_ns() - t0 <= limit_ns) {
+  }
+  if (!__all_sync(0xffffffffu, ok)) late_received(bar, abort_flag, err_bit);
+}
 // Arrive on an mbarrier given by its shared::cluster address (possibly the peer's).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)

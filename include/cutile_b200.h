@@ -431,6 +431,14 @@ int ctb_fill_normal(void* ptr, int32_t dtype, int64_t n, uint64_t seed,
  * its kernels have no bounded waits). */
 int ctb_selftest_wait_timeout(int64_t limit_ns, int* status, void* stream);
 
+/* Launches a cluster of two CTAs: one sends 32 words to the other's shared
+ * memory `delay_ns` after the start and leaves, the other waits for them,
+ * giving up after `limit_ns` (both 1..1e9). `status` (device memory, 2 ints):
+ * [0] = the words that were there when the waiting CTA went on, 32 also where
+ * its wait gave up (it stays until the sends have landed), [1] = 1 when the
+ * wait gave up; the next ctb_check_device then returns CTB_ERR_TIMEOUT. */
+int ctb_selftest_late_sender(int64_t limit_ns, int64_t delay_ns, int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
