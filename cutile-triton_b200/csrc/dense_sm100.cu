@@ -26,6 +26,7 @@
 #include "sm100_ptx.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -912,9 +913,20 @@ static int pair_mode() {
   return mode;
 }
 
+// Tile rows (256: the pair kernel) and split that the self-tests ask for, rows << 8
+// | split; 0: none asked for.
+static std::atomic<int> g_asked{0};
+
 static Plan choose_plan(const Product& p, int sms, int pairs) {
   const double out_bytes = (1 + (p.Z ? 1 : 0) + (p.R ? 1 : 0)) * 2.0 * p.rows * p.cols;
   Plan best = {0, 1};
+  if (const int asked = g_asked.load(std::memory_order_relaxed)) {
+    const int BN = asked >> 8, kb = (int)(((int64_t)p.depth + BK - 1) / BK);
+    if (BN == 256 && pairs > 0) return best;
+    // A tile of row-major-k rows is 64 wide at least; each CTA has two k-blocks at least.
+    return {std::max(p.p_mn ? 64 : 16, std::min(BN, 128)),
+            std::max(1, std::min(asked & 255, kb / 2))};
+  }
   double us = pairs > 0 ? pair_us(p, pairs) : 1e30;
   const int mode = pair_mode();
   if (mode == 1 && pairs > 0) return best;
@@ -1041,3 +1053,14 @@ template int product_sm100<__nv_bfloat16>(const Product&, int, cudaStream_t);
 
 int dense_take_device_error(unsigned int* out) { return take_device_error(out); }
 }  // namespace ctb
+
+extern "C" int ctb_selftest_dense_plan(int32_t rows, int32_t split) {
+  using namespace ctb;
+  clear_error();
+  if (rows != 0 && rows != 16 && rows != 32 && rows != 64 && rows != 128 && rows != 256)
+    return set_error(CTB_ERR_ARG, "ctb_selftest_dense_plan: rows must be 0, 16, 32, 64, 128 or 256");
+  if (rows != 0 && (split < 1 || split > 8))
+    return set_error(CTB_ERR_ARG, "ctb_selftest_dense_plan: split must be 1 to 8");
+  dense::g_asked = rows ? rows << 8 | split : 0;
+  return CTB_OK;
+}

@@ -113,6 +113,7 @@ SIGNATURES = {
     "ctb_fill_normal": [_P, _I32, _I64, _U64, _U64, _D, _D, _P],
     "ctb_selftest_wait_timeout": [_I64, _P, _P],
     "ctb_selftest_late_sender": [_I64, _I64, _P, _P],
+    "ctb_selftest_dense_plan": [_I32, _I32],
 }
 
 _lib = None

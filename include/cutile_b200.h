@@ -417,7 +417,7 @@ int ctb_fill_uniform(void* ptr, int32_t dtype, int64_t n, uint64_t seed,
 int ctb_fill_normal(void* ptr, int32_t dtype, int64_t n, uint64_t seed,
                     uint64_t offset, double mean, double std, void* stream);
 
-/* ---- failure-path self-test (test plumbing, not a cuTile op) ------------- */
+/* ---- self-tests (test plumbing, not a cuTile op) -------------------------- */
 
 /* Launches one CTA whose warp 0 holds 32 TMEM columns and waits on an
  * mbarrier that nothing arrives on, giving up after `limit_ns` (1..1e9);
@@ -438,6 +438,13 @@ int ctb_selftest_wait_timeout(int64_t limit_ns, int* status, void* stream);
  * its wait gave up (it stays until the sends have landed), [1] = 1 when the
  * wait gave up; the next ctb_check_device then returns CTB_ERR_TIMEOUT. */
 int ctb_selftest_late_sender(int64_t limit_ns, int64_t delay_ns, int* status, void* stream);
+
+/* The dense layer's products of this process from here on: on tiles of `rows`
+ * rows (16, 32, 64 or 128) with k split over `split` (1..8) CTAs, or with rows
+ * = 256 on the CTA-pair kernel, instead of what the model of their times
+ * takes; where a product cannot have the tile or split, on the next that it
+ * can. rows = 0: as the model takes them. */
+int ctb_selftest_dense_plan(int32_t rows, int32_t split);
 
 #ifdef __cplusplus
 }
