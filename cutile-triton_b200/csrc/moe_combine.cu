@@ -6,8 +6,10 @@
 // y was never written and is not read.
 //
 // Both are bound by HBM: every row of y is moved once. Forward: one thread per
-// 16 bytes of a token's row, whose topk loads (and the residual's) are all in
-// flight before the first is used; sums in Float32, rounded once. Gradient:
+// 16 bytes of a token's row (per element where rows are no 16-byte runs: 4096
+// tokens x 2 x 4095 take 91 us, x 4096 21), whose loads, up to 8 slots' and the
+// residual's, are all in flight before the first is used; with more slots their
+// ids and rows are loaded in turn. Sums in Float32, rounded once. Gradient:
 // one warp per slot, the slots of a token in neighbouring warps, so dout comes
 // from HBM once and from L1 for the other slots; the warp's lanes keep the dot
 // product's partial sums and join them with shuffles (fixed order). 16384 tokens
@@ -234,12 +236,17 @@ template <typename T, int W>
 int combine_launch(const CombineArgs<T>& a, cudaStream_t st) {
   const int64_t grid = (a.items + COMBINE_THREADS - 1) / COMBINE_THREADS;
   if (grid > 0x7fffffff) return set_error(CTB_ERR_SHAPE, "moe_combine: too many elements");
+  // Up to 8 slots by straight code, any other number in a loop: 4096 tokens of 4096
+  // columns 26 us against 36 for 3 slots, 53 against 70 for 8.
   auto k = moe_combine_kernel<T, W, 0>;
   switch (a.topk) {
     case 1: k = moe_combine_kernel<T, W, 1>; break;
     case 2: k = moe_combine_kernel<T, W, 2>; break;
+    case 3: k = moe_combine_kernel<T, W, 3>; break;
     case 4: k = moe_combine_kernel<T, W, 4>; break;
+    case 5: k = moe_combine_kernel<T, W, 5>; break;
     case 6: k = moe_combine_kernel<T, W, 6>; break;
+    case 7: k = moe_combine_kernel<T, W, 7>; break;
     case 8: k = moe_combine_kernel<T, W, 8>; break;
     default: break;
   }
