@@ -97,7 +97,14 @@ float real(PyObject* o, const char* what) {
   }
   return (float)v;
 }
-bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject* o, const char* what) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) {
+    PyErr_Clear();
+    refuse(CTB_ERR_ARG, std::string(what) + ": expected a truth value");
+  }
+  return v == 1;
+}
 
 // A call's first matrix, whose shape, dtype and device the others are held to.
 const Tensor& rows(PyObject* o, const char* what) {
@@ -256,7 +263,8 @@ PyObject* dense_bwd(PyObject* const* v) {
     pre = ptr(z);
     ldz = ld(z);
   }
-  const bool need[3] = {truth(v[8]), truth(v[9]), truth(v[10])};
+  const bool need[3] = {truth(v[8], "dense_bwd: need_dA"), truth(v[9], "dense_bwd: need_dB"),
+                        truth(v[10], "dense_bwd: need_dbias")};
   if (need[0] && given(v[5])) matrix(v[5], l.K, l.M, l.dt, l.dev, "dense_bwd: dA_t");
   if (need[1] && given(v[6])) matrix(v[6], l.N, l.K, l.dt, l.dev, "dense_bwd: dB_t");
   if (need[2] && given(v[7])) vector(v[7], l.M, at::kFloat, l.dev, "dense_bwd: dbias");
@@ -304,12 +312,13 @@ PyObject* moe_route(PyObject* const* v) {
   if (given(v[9])) packed(v[9], T, topk, at::kFloat, dev, "moe_route: weights");
   if (given(v[10])) packed(v[10], T, topk, at::kInt, dev, "moe_route: ids");
   const float scale = real(v[8], "moe_route: scale");
+  const int renorm = truth(v[7], "moe_route: renorm") ? 1 : 0;
   On on(dev);
   Tensor w = given(v[9]) ? THPVariable_Unpack(v[9]) : new_matrix(T, topk, at::kFloat, dev);
   Tensor i = given(v[10]) ? THPVariable_Unpack(v[10]) : new_matrix(T, topk, at::kInt, dev);
   check(lib.ctb_moe_route(dtype_code(x.scalar_type()), ptr(x), bias, static_cast<float*>(ptr(w)),
                           static_cast<int32_t*>(ptr(i)), T, E, topk, ld(x), score, groups, kept,
-                          top, truth(v[7]) ? 1 : 0, scale, on.stream));
+                          top, renorm, scale, on.stream));
   return pair_of(std::move(w), std::move(i));
 }
 
@@ -324,11 +333,12 @@ PyObject* moe_route_bwd(PyObject* const* v) {
   if (given(v[6])) matrix(v[6], T, E, x.scalar_type(), dev, "moe_route_bwd: dlogits");
   const int score = (int)integer(v[3], "moe_route_bwd: score");
   const float scale = real(v[5], "moe_route_bwd: scale");
+  const int renorm = truth(v[4], "moe_route_bwd: renorm") ? 1 : 0;
   On on(dev);
   Tensor dx = given(v[6]) ? THPVariable_Unpack(v[6]) : new_matrix(T, E, x.scalar_type(), dev);
   check(lib.ctb_moe_route_bwd(dtype_code(x.scalar_type()), static_cast<const float*>(ptr(dw)),
                               ptr(x), static_cast<const int32_t*>(ptr(i)), ptr(dx), T, E, topk,
-                              ld(x), ld(dx), score, truth(v[4]) ? 1 : 0, scale, on.stream));
+                              ld(x), ld(dx), score, renorm, scale, on.stream));
   return THPVariable_Wrap(std::move(dx));
 }
 
