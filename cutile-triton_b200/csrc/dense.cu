@@ -42,8 +42,8 @@ __global__ void __launch_bounds__(256) product_empty_kernel(const Product p) {
 // ---- operands that TMA cannot address ----------------------------------------------------
 int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
 // Copies have lines of whole 128-byte rows: lines that TMA can address but that
-// start inside a 128-byte line load half as fast again (768 x 1000 x 1000 10.6 us,
-// 768 x 1024 x 1024 7.2).
+// start inside a 128-byte line load more slowly (768 x 1000 x 1000, where nothing is
+// copied, 12.5 us; 768 x 1024 x 1024 7.4).
 int64_t pitch(int64_t n) { return (n + 63) / 64 * 64; }
 
 // A matrix of `lines` lines of `len` contiguous elements is addressable where
@@ -55,7 +55,8 @@ int64_t packed_bytes(int64_t lines, int64_t len) { return round256(2 * lines * p
 
 // Copies lines of 16-bit elements to lines pitch(len) apart; one thread per 16
 // bytes of the result. Both operands of a product in one launch (the grid's y).
-// 4097 x 8193: 26 us for 134 MB moved (20 us at the copy rate).
+// One row by 4097 x 8193: 40 us, of which the copy of the weight (134 MB moved, 20 us
+// at the copy rate) is 27; 13 us where the weight's lines are aligned.
 struct Pack {
   const uint16_t* src;
   uint4* dst;
@@ -125,9 +126,10 @@ int product(const Product& p, int sms, cudaStream_t st) {
 // of one strip, two of them in flight per warp; a lane keeps its columns' sums.
 // The strip's rows are split into spans so that every SM has several CTAs'
 // worth; spans are summed afterwards in order, so the result does not depend on
-// the schedule. 4096 x 16384 (268 MB read, 41 us at the copy rate): 46 us with
-// relu, 66 with gelu (18 instructions an element; 2 rows in flight at 4 CTAs an
-// SM measured better than 1, and than 4 rows at 2 or 3 CTAs: 68-72 us).
+// the schedule. Bias gradient of 4096 x 16384 (268 MB read, no dZ written, 41 us
+// at the copy rate): 45 us with relu, 53 silu, 58 gelu_tanh, 67 gelu (18
+// instructions an element; 2 rows in flight at 4 CTAs an SM measured better than
+// 1, and than 4 rows at 2 or 3 CTAs: 68-72 us).
 constexpr int SLOPE_THREADS = 256, SLOPE_WARPS = SLOPE_THREADS / 32, SLOPE_FLIGHT = 2;
 constexpr int SLOPE_CTAS = 16 * 148;
 

@@ -69,8 +69,8 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 // Evaluated on pairs: the packed f32x2 instructions take one issue slot for two
 // elements, and an epilogue's slots are what an activation costs (its power too).
 // ex2.approx.ftz and rcp.approx.ftz are documented to 2 ulp and 1 ulp; results
-// below the normal range become 0, which is below half a step of any output
-// they are added to or round to.
+// below the normal range become 0. That shows in BFloat16 only, in values of
+// 1e-36 and below: silu(-88), -5e-37 exactly, is 0 here.
 using f2 = uint64_t;
 __device__ __forceinline__ f2 mk2(float a, float b) {
   f2 r;
@@ -132,8 +132,8 @@ __device__ __forceinline__ f2 logistic_ex2(f2 v) {
 // is smooth in t over (0, 1]; this is its polynomial of degree 6 with the least
 // largest relative error (1.8e-6, by reweighted least squares on 4400 points
 // of [0, 40]). In 32 bits z * Phi(z) is within 4e-7 of the exact value for |z| <
-// 12. A call of erfcf instead made a 4096 x 4096 x 1024 layer take 115 us
-// against 51 us without an activation.
+// 12. A call of erfcf instead makes a 4096 x 4096 x 1024 bf16 layer take 60 us,
+// against 33 us, and 29 without an activation.
 __device__ __forceinline__ f2 normal_tail(f2 a, f2* density) {
   const f2 e = ex2_2(mul2(mul2(a, a), all2(-0.5f * kLog2e)));
   const f2 t = rcp_2(fma2(a, all2(0.273f), all2(1.f)));

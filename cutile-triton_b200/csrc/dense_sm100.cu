@@ -11,8 +11,8 @@
 // the row's owner) and add them in rank order, each finishing (bias, activation,
 // residual, rounding) its share of the tile. No workspace, no atomics, the same
 // result every time. Bound by HBM from some tens of MB of weight up (37 x 14336 x
-// 4096 bf16: 23.4 us, 5.1 TB/s), below that by set-up, first load and the joining
-// of the sums (1 x 4096 x 4096 f16: 8.0 us, 4.2 TB/s; 64 x 1024 x 1024: 4.1 us).
+// 4096 bf16: 23 us, 5.2 TB/s), below that by set-up, first load and the joining
+// of the sums (1 x 4096 x 4096 f16: 8.0 us, 4.2 TB/s; 64 x 1024 x 1024: 4.2 us).
 //
 // product_pair_kernel: 256 x 256 tiles over two SMs (tcgen05 cta_group::2),
 // persistent, for products with tiles enough to fill the GPU. Here the rows of D
@@ -20,8 +20,9 @@
 // columns of one row, which move through swizzled shared memory as 16-byte
 // pieces and in and out of it by TMA, and the bias is the same for all lanes.
 // Bound by the tensor pipe, in long runs by the power cap: 8192 x 14336 x 4096 bf16
-// with bias, gelu and Z 751 us (1281 TFLOP/s) back to back, 1500 to 1570 TFLOP/s
-// without an epilogue in a burst; 4096 x 4096 x 1024 30 us.
+// with bias, gelu and Z 726 to 751 us back to back (1325 to 1281 TFLOP/s, from one
+// GPU to another), 673 without an epilogue (1430); 4096 x 4096 x 1024 bf16 29 us, 33
+// with gelu, 41 with bias, gelu and Z.
 #include "dense.cuh"
 #include "sm100_ptx.cuh"
 
@@ -876,9 +877,15 @@ static bool rows16(const void* p, int64_t ld, int rows) {
 
 // ---- which kernel, tile and split ------------------------------------------------------
 // A model of the two kernels' times in microseconds. Its numbers make the choice
-// by it the fastest one measured as nearly as possible over 1658 runs (150
-// products of 1 to 6000 rows, 256 to 14336 columns, 300 to 14336 k, each with
-// every tile and split): it takes 1.2% longer than the best, 20% at worst. A split
+// by it the fastest one measured as nearly as possible over 1658 runs of forward
+// products with nothing in their epilogue (150 of f16, 1 to 6000 rows, 256 to 14336
+// columns, 300 to 14336 k, each with every tile and split): it takes 1.2% longer
+// than the best, 20% at worst. They are a fit and no rates of the chip (9.66 TB/s,
+// say, is above what HBM gives). On 48 other products in bf16 (1 to 4096 rows, 256
+// to 4096 columns, 8 to 8192 k) its choice took longer than the best by, on average
+// and at worst: forward 4% and 12%, with gelu and Z 7% and 29% (513 x 4096 x 2048 on
+// the pair kernel, whose epilogue no longer hides there), dB 4% and 12%, dA 1% and
+// 3%. Splits of 5 and 7 are left out: on these they beat the rest once, by 1.5%. A split
 // CTA takes its k-blocks at 79 GB/s, alone or beside another on its SM; 256 CTAs
 // in clusters are sure to be resident at once, 296 single ones; more row tiles
 // read the weight again from L2. A pair takes 0.3 us a k-block and 3.1 us a tile.

@@ -7,14 +7,14 @@
 //
 // Both are bound by HBM: every row of y is moved once. Forward: one thread per
 // 16 bytes of a token's row (per element where rows are no 16-byte runs: 4096
-// tokens x 2 x 4095 take 91 us, x 4096 21), whose loads, up to 8 slots' and the
+// tokens x 2 x 4095 take 93 us, x 4096 21), whose loads, up to 8 slots' and the
 // residual's, are all in flight before the first is used; with more slots their
 // ids and rows are loaded in turn. Sums in Float32, rounded once. Gradient:
 // one warp per slot, the slots of a token in neighbouring warps, so dout comes
 // from HBM once and from L1 for the other slots; the warp's lanes keep the dot
 // product's partial sums and join them with shuffles (fixed order). 16384 tokens
-// x 2 x 4096 f16 with residual: 81 us, the copy rate (6.6 TB/s); gradients of 4099
-// x 8 x 2048 bf16: 48.7 us, 5.9 TB/s.
+// x 2 x 4096 f16 with residual: 79 to 82 us, the copy rate (6.6 TB/s); gradients of
+// 4099 x 8 x 2048 bf16: 48 to 49 us, 5.9 TB/s (97 where N is 2047).
 #include "ctb_common.cuh"
 
 #include <algorithm>

@@ -11,21 +11,27 @@
 // An expert whose logit is -inf or NaN, or whose c is, cannot be chosen; a
 // place that no expert is left for gets id -1 and weight 0.
 //
-// The choice is the one of exact arithmetic. Without a bias the experts of a
-// row rank as their logits do, which needs no arithmetic. With a bias, and
-// between groups, c is computed in 32 bits first; where two values that decide
-// the order are closer than those 32 bits tell apart (about one row in a
-// thousand), the candidates, or where groups are in doubt the whole row, are
-// ranked again in 64 bits.
+// The choice is the one of Float64. Without a bias the experts of a row rank as
+// their logits do, which needs no arithmetic. With a bias, and between groups, c
+// is computed in 32 bits first; where two values that decide the order are
+// closer than those 32 bits tell apart, the candidates, or where groups are in
+// doubt the whole row, are ranked again in 64 bits (where those cannot tell them
+// apart either, as sigmoids of 40 and 50, it is a tie). How often that happens
+// is up to the inputs: for 8 of 256 experts by sigmoid, one row in 2000 for f32
+// logits of deviation 1.5 under a bias of deviation 0.1; under a zero bias a third
+// of the rows for the same logits in bf16, half of them for f32 logits of
+// deviation 5, and every row for deviation 8, whose sigmoids saturate.
 //
 // A row belongs to LANES lanes of a warp, NV neighbouring experts to a lane, so
 // that a tie goes to the first lane and the first register. Each choice is one
 // maximum over the lanes and a rescan of the winner's NV registers. Rows of up
 // to 64 experts take 8 lanes (four rows per warp).
 //
-// Bound by instruction issue (IPC 2.5 to 3.2), not by HBM: 65536 x 256 f32 takes 39
-// us without a bias and 62 with bias and groups (800 instructions a row) against
-// 10 at the copy rate; 16384 rows 16.5 us.
+// Bound by instruction issue (IPC 2.7), not by HBM: 65536 x 256 f32 takes 40
+// us without a bias and 61 with bias and groups (840 instructions a row) against
+// 10 at the copy rate; 16384 rows 12 and 17 to 18. The 64-bit ranking shows: 16384 x
+// 256 with 4 of 8 groups and a zero bias takes 17 us for logits of deviation 1.5
+// (24 in bf16), 26 for 5, 55 for 8; by softmax 21, 26 and 46, and 42 for 0.05.
 #include "ctb_common.cuh"
 
 #include <algorithm>
@@ -643,8 +649,9 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(const T* x,
 //   sigmoid         dx = g s (1 - s)                     chosen experts only
 //   sigmoid, renorm dx = p (1 - s) * (g - sum(g p))      chosen experts only
 // One pass: the row (plain softmax) or the chosen logits are read, the whole
-// row of dx is written once. 65536 x 256 f32 plain softmax: 38 us, 20 at the copy
-// rate; 16384 x 64: 4.8 us with its launch.
+// row of dx is written once. 65536 x 256 f32 plain softmax, 8 chosen: 39 us, 20 at
+// the copy rate, beside which a lane compares its 8 registers with each of the 8
+// places and takes 8 expf; 16384 x 64: 4.8 us with its launch.
 // -----------------------------------------------------------------------------
 struct RouteBwdArgs {
   const float* dweights;

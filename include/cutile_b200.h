@@ -363,7 +363,11 @@ typedef enum { CTB_SCORE_SOFTMAX = 0, CTB_SCORE_SIGMOID = 1 } ctb_score;
  * expert is left for gets id -1 (which ctb_moe_align_i32 does not list) and
  * weight 0, so a row of -inf routes a padding token nowhere. A logit of +inf
  * gives NaN weights under softmax, as the formula does. The choice is that of
- * exact arithmetic, also where c differs by less than Float32 resolves.
+ * c in Float64, also where c differs by less than Float32 resolves; without a
+ * bias the experts of a row, or of its groups kept, rank as their logits.
+ * The weights are Float32 with a relative error of a few 2^-24, and of 2e-7
+ * more for each unit that a chosen logit lies below the row's largest (sigmoid:
+ * below 0).
  * weights and ids: T x topk, contiguous. E <= 256, topk <= 32. */
 int ctb_moe_route(int32_t dtype, const void* logits, const float* bias, float* weights,
                   int32_t* ids, int32_t T, int32_t E, int32_t topk, int64_t ldx, int32_t score,
