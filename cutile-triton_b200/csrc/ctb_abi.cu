@@ -32,17 +32,12 @@ static __int128 floor_div(__int128 a, __int128 b) {  // b > 0
   return a % b < 0 ? q - 1 : q;
 }
 
-bool overlap(const Lines& x, const Lines& y) {
+bool lines_meet(const Lines& x, const Lines& y) {
   const Lines &a = x.rows <= y.rows ? x : y, &b = x.rows <= y.rows ? y : x;
-  if (!a.p || !b.p || a.rows <= 0 || a.len <= 0 || b.len <= 0) return false;
-  const __int128 d = (__int128)reinterpret_cast<uintptr_t>(a.p) -
-                     (__int128)reinterpret_cast<uintptr_t>(b.p);
+  const __int128 d = (__int128)a.begin - (__int128)b.begin;
   const __int128 pa = a.rows > 1 ? a.pitch : 0, pb = b.rows > 1 ? b.pitch : b.len;
-  // Lines of `a` that reach into the bytes from b's first to its last.
-  const __int128 end_b = (b.rows - 1) * pb + b.len;
-  if (d + (a.rows - 1) * pa + a.len <= 0 || d >= end_b) return false;
-  // Whether one of the lines from..to (in bytes from b's start) meets a line of b:
-  // the first line of b that ends after `at` must start before at + a.len.
+  // Whether a line of `a`, `at` bytes from b's start, meets a line of b: the first line
+  // of b that ends after `at` must start before at + a.len.
   const auto meets = [&](__int128 at) {
     __int128 j = floor_div(at - b.len, pb) + 1;
     if (j < 0) j = 0;

@@ -38,15 +38,27 @@ inline int launch_status(const char* what) {
 struct Lines {
   const void* p;
   int64_t rows, len, pitch;
+  uintptr_t begin, end;  // all bytes from the first line's to the last's; both 0 for nothing
 };
 // A matrix of elements of `size` bytes whose lines are `ld` elements apart.
 inline Lines lines_of(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t size) {
-  return {p, rows, cols * size, rows > 1 ? ld * size : cols * size};
+  Lines l = {p, rows, cols * size, rows > 1 ? ld * size : cols * size, 0, 0};
+  if (!p || rows <= 0 || cols <= 0) return l;
+  l.begin = reinterpret_cast<uintptr_t>(p);
+  uintptr_t bytes;
+  if (__builtin_mul_overflow((uintptr_t)(rows - 1), (uintptr_t)l.pitch, &bytes) ||
+      __builtin_add_overflow(bytes, l.begin + (uintptr_t)l.len, &l.end))
+    l.end = UINTPTR_MAX;
+  return l;
 }
-inline Lines bytes_of(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+inline Lines bytes_of(const void* p, int64_t bytes) { return lines_of(p, 1, bytes, bytes, 1); }
+// Whether lines whose bytes from first to last meet share any.
+bool lines_meet(const Lines& a, const Lines& b);
 // Whether any byte belongs to both. Lines that lie between one another's (columns
 // of one wider buffer, every other row of it) do not overlap.
-bool overlap(const Lines& a, const Lines& b);
+inline bool overlap(const Lines& a, const Lines& b) {
+  return a.begin < b.end && b.begin < a.end && lines_meet(a, b);
+}
 inline bool apart(const Lines& a, std::initializer_list<Lines> others) {
   for (const Lines& o : others)
     if (overlap(a, o)) return false;
