@@ -20,7 +20,7 @@
 // columns of one row, which move through swizzled shared memory as 16-byte
 // pieces and in and out of it by TMA, and the bias is the same for all lanes.
 // Bound by the tensor pipe, in long runs by the power cap: 8192 x 14336 x 4096 bf16
-// with bias, gelu and Z 726 to 751 us back to back (1325 to 1281 TFLOP/s, from one
+// with bias, gelu and Z 726 to 756 us back to back (1325 to 1272 TFLOP/s, from one
 // GPU to another), 673 without an epilogue (1430); 4096 x 4096 x 1024 bf16 29 us, 33
 // with gelu, 41 with bias, gelu and Z.
 #include "dense.cuh"
